@@ -307,6 +307,45 @@ int pai_add_layernorm_bf16(const void *x, const void *y, const void *gamma, cons
 int pai_gelu_bf16(const void *x, void *out, long long n, void *stream);
 
 /* ---------------------------------------------------------------------------------------
+ * The products of the feed-forward block (the reference runs them as PyTorch operators: `MLP.forward`,
+ * utils/model_utils/base_modules/base_modules.py:46-52, and the residual of `Encoder.forward`, old/old_scripts/encoder.py:39-41), each one
+ * kernel with its epilogue, and their gradients:
+ *   pai_linear_fwd   y = act(x w^T + bias) + residual
+ *   pai_gated_fwd    h = act(x w_gate^T + bias_gate) * (x w_up^T + bias_up)
+ *   pai_linear_bwd   dz = dy act'(z):  dx = dz w,  dw = dz^T x,  db = column sums of dz   (the residual's gradient is dy itself)
+ *   pai_gated_bwd    dg = dh u act'(g), du = dh act(g):  dx = dg w_gate + du w_up,  dw_* = d*^T x,  db_* = column sums
+ * x [M, K], w, w_gate, w_up [N, K], y, h, residual, dy, dh [M, N], dx [M, K], dw* [N, K] contiguous, all of the 16-bit type `dtype`
+ * (enum pai_dtype) with contiguous columns and the given row pitch in elements; bias* and db* [N] of that type, or fp32 when bias_fp32 != 0.
+ * Any of bias*, residual, dx, dw*, db* may be NULL (left out).  act: enum pai_act.  Products, epilogue and sums are fp32; every output is
+ * rounded once, and dz (dg, du) once to `dtype` in between.
+ * Operands of the products (x and w*; dy of pai_linear_bwd without an activation) need 16-byte aligned rows: base 16-byte aligned, pitch a
+ * multiple of 8 elements (pai_copy_rows16 makes such a copy).  y, h, residual, dx, and dy otherwise, may have any alignment and pitch.
+ *   saved      NULL (inference), or pai_dense_saved_bytes(M, N, gated) bytes, 16-byte aligned: the pre-activations for the backward call,
+ *              in a layout of the library's own; pai_linear_bwd without an activation needs none.
+ *   workspace  pai_dense_bwd_workspace_bytes(M, N, gated) bytes, 256-byte aligned.
+ * Limits: M < 2^31 - 2^16, N and K <= 2^20.  Results are the same bits from call to call.
+ *   pai_copy_rows16  dst[r, c] = src[r, c] for rows of 16-bit elements of any alignment into 16-byte aligned rows; columns up to the next
+ *                    multiple of 8 are written as zeros.
+ */
+enum pai_dtype { PAI_BF16 = 0, PAI_FP16 = 1 };
+enum pai_act { PAI_ACT_NONE = 0, PAI_ACT_GELU = 1 /* erf form */, PAI_ACT_SILU = 2, PAI_ACT_RELU = 3, PAI_ACT_SIGMOID = 4 };
+#define PAI_DENSE_MAX_ROWS 2147418111ll
+#define PAI_DENSE_MAX_WIDTH 1048576
+size_t pai_dense_saved_bytes(long long M, int N, int gated);
+size_t pai_dense_bwd_workspace_bytes(long long M, int N, int gated);
+int pai_linear_fwd(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, int bias_fp32, const void *residual, int64_t ldr,
+                   void *y, int64_t ldy, void *saved, long long M, int N, int K, int act, int dtype, void *stream);
+int pai_gated_fwd(const void *x, int64_t ldx, const void *w_gate, int64_t ldwg, const void *w_up, int64_t ldwu, const void *bias_gate,
+                  const void *bias_up, int bias_fp32, void *h, int64_t ldh, void *saved, long long M, int N, int K, int act, int dtype, void *stream);
+int pai_linear_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *saved, void *dx, int64_t lddx,
+                   void *dw, void *db, int bias_fp32, void *workspace, size_t workspace_bytes, long long M, int N, int K, int act, int dtype,
+                   void *stream);
+int pai_gated_bwd(const void *dh, int64_t lddh, const void *x, int64_t ldx, const void *w_gate, int64_t ldwg, const void *w_up, int64_t ldwu,
+                  const void *saved, void *dx, int64_t lddx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, int bias_fp32, void *workspace,
+                  size_t workspace_bytes, long long M, int N, int K, int act, int dtype, void *stream);
+int pai_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld_dst, long long rows, int cols, void *stream);
+
+/* ---------------------------------------------------------------------------------------
  * Nearest-neighbour graph and radial-basis edge features: FeaturizeProtein.get_neighbors and the tensor part of
  * FeaturizeProtein.get_edges (utils/model_utils/gnn/gnn.py:97-117 and :119-131), which the reference evaluates in
  * PyTorch through an N x N distance matrix, torch.topk and a [Z,N,K,4,4,R] broadcast (no reference FFI to replace).

@@ -41,6 +41,17 @@ SIGNATURES = {
                                 c_int, c_int, c_int, c_int, c_void_p]),
     "pai_add_layernorm_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, ctypes.c_longlong, c_int, c_float, c_void_p]),
     "pai_gelu_bf16": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, c_void_p]),
+    "pai_dense_saved_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "pai_dense_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "pai_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                               c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "pai_gated_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p,
+                              c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "pai_linear_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_int,
+                               c_void_p, c_size_t, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "pai_gated_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
+                              c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "pai_copy_rows16": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
     "pai_knn_neighbors": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
     "pai_edge_rbf": (c_int, [c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_float, c_void_p,
                              c_int, c_int, c_int, c_int, c_int, c_void_p]),

@@ -2,6 +2,7 @@
 // the kernels are header files so that the device status word needs no relocatable device code.
 #include "common.cuh"
 
+#include "dense_host.cuh"
 #include "geoattn_bwd.cuh"
 #include "encoder_ops.cuh"
 #include "neighbors.cuh"
@@ -113,7 +114,7 @@ __global__ void __launch_bounds__(256) sfu_peak_kernel(int iters, float seed) {
 
 extern "C" {
 
-int pai_abi_version(void) { return 6; }  // 6: balanced attention schedules (5: WE flags, batch plan, query-row ranges, test-only entries)
+int pai_abi_version(void) { return 7; }  // 7: feed-forward products (6: balanced attention schedules 5: WE flags, batch plan, query-row ranges, test-only entries)
 
 const char *pai_status_str(int status) {
     switch (status) {
@@ -613,6 +614,146 @@ int pai_gelu_bf16(const void *x, void *out, long long n, void *stream) {
     int sms = 0;
     if (int e = current_device_sms(&sms)) return e;
     return pai::gelu_bf16_launch(x, out, n, sms, (cudaStream_t)stream);
+}
+
+// ---- feed-forward products -----------------------------------------------------------------------
+namespace {
+int check_dense_sizes(long long M, int N, int K, int act, int dtype) {
+    if (M < 0 || M > PAI_DENSE_MAX_ROWS || N < 1 || N > PAI_DENSE_MAX_WIDTH || K < 1 || K > PAI_DENSE_MAX_WIDTH) return PAI_ERR_BAD_SHAPE;
+    if (act < 0 || act >= pai::ACT_COUNT || (dtype != PAI_BF16 && dtype != PAI_FP16)) return PAI_ERR_UNSUPPORTED;
+    return 0;
+}
+// rows that TMA reads: 16-byte aligned base and pitch, no overlap
+int check_dense_operand(const void *p, int64_t ld, long long rows, int cols) {
+    if (!p) return PAI_ERR_NULL_POINTER;
+    if (rows > 1 && (ld < cols || ld >= (1ll << 38))) return PAI_ERR_BAD_SHAPE;
+    if (!aligned(p, 16) || (rows > 1 && (ld & 7) != 0)) return PAI_ERR_MISALIGNED;
+    return 0;
+}
+// rows that plain loads and stores touch
+int check_dense_rows(const void *p, int64_t ld, long long rows, int cols, bool written) {
+    if (!p) return PAI_ERR_NULL_POINTER;
+    if (rows > 1 && (ld < (written ? cols : 0) || ld >= (1ll << 38))) return PAI_ERR_BAD_SHAPE;
+    return aligned(p, 2) ? 0 : PAI_ERR_MISALIGNED;
+}
+}  // namespace
+
+size_t pai_dense_saved_bytes(long long M, int N, int gated) {
+    if (M < 1 || M > PAI_DENSE_MAX_ROWS || N < 1 || N > PAI_DENSE_MAX_WIDTH) return 0;
+    return (gated ? 2 : 1) * pai::saved_bytes_f32(M, N);
+}
+
+size_t pai_dense_bwd_workspace_bytes(long long M, int N, int gated) {
+    if (M < 1 || M > PAI_DENSE_MAX_ROWS || N < 1 || N > PAI_DENSE_MAX_WIDTH) return 0;
+    return pai::dense_bwd_workspace(M, N, gated ? 2 : 1);
+}
+
+int pai_linear_fwd(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, int bias_fp32, const void *residual, int64_t ldr,
+                   void *y, int64_t ldy, void *saved, long long M, int N, int K, int act, int dtype, void *stream) {
+    if (int e = check_dense_sizes(M, N, K, act, dtype)) return e;
+    if (int e = check_dense_operand(x, ldx, M, K)) return e;
+    if (int e = check_dense_operand(w, ldw, N, K)) return e;
+    if (int e = check_dense_rows(y, ldy, M, N, true)) return e;
+    if (residual)
+        if (int e = check_dense_rows(residual, ldr, M, N, false)) return e;
+    if ((bias && !aligned(bias, bias_fp32 ? 4 : 2)) || (saved && !aligned(saved, 16))) return PAI_ERR_MISALIGNED;
+    if (int e = require_sm100()) return e;
+    if (M == 0) return PAI_OK;
+    int sms = 0;
+    if (int e = current_device_sms(&sms)) return e;
+    const pai::DenseOperand ws[2] = {{w, ldw}, {nullptr, 0}};
+    const void *const bs[2] = {bias, nullptr};
+    return pai::dense_forward({x, ldx}, ws, bs, bias_fp32 != 0, {residual, ldr}, y, ldy, saved, M, N, K, act, dtype == PAI_FP16, sms,
+                              (cudaStream_t)stream);
+}
+
+int pai_gated_fwd(const void *x, int64_t ldx, const void *w_gate, int64_t ldwg, const void *w_up, int64_t ldwu, const void *bias_gate,
+                  const void *bias_up, int bias_fp32, void *h, int64_t ldh, void *saved, long long M, int N, int K, int act, int dtype, void *stream) {
+    if (int e = check_dense_sizes(M, N, K, act, dtype)) return e;
+    if (int e = check_dense_operand(x, ldx, M, K)) return e;
+    if (int e = check_dense_operand(w_gate, ldwg, N, K)) return e;
+    if (int e = check_dense_operand(w_up, ldwu, N, K)) return e;
+    if (int e = check_dense_rows(h, ldh, M, N, true)) return e;
+    const size_t ba = bias_fp32 ? 4 : 2;
+    if ((bias_gate && !aligned(bias_gate, ba)) || (bias_up && !aligned(bias_up, ba)) || (saved && !aligned(saved, 16))) return PAI_ERR_MISALIGNED;
+    if (int e = require_sm100()) return e;
+    if (M == 0) return PAI_OK;
+    int sms = 0;
+    if (int e = current_device_sms(&sms)) return e;
+    const pai::DenseOperand ws[2] = {{w_gate, ldwg}, {w_up, ldwu}};
+    const void *const bs[2] = {bias_gate, bias_up};
+    return pai::dense_forward({x, ldx}, ws, bs, bias_fp32 != 0, {nullptr, 0}, h, ldh, saved, M, N, K, act, dtype == PAI_FP16, sms,
+                              (cudaStream_t)stream);
+}
+
+int pai_linear_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, const void *w, int64_t ldw, const void *saved, void *dx, int64_t lddx,
+                   void *dw, void *db, int bias_fp32, void *workspace, size_t workspace_bytes, long long M, int N, int K, int act, int dtype,
+                   void *stream) {
+    if (int e = check_dense_sizes(M, N, K, act, dtype)) return e;
+    if (M < 1) return PAI_ERR_BAD_SHAPE;
+    if (act == pai::ACT_NONE && (dx || dw)) {  // dy itself is an operand
+        if (int e = check_dense_operand(dy, lddy, M, N)) return e;
+    } else {
+        if (int e = check_dense_rows(dy, lddy, M, N, false)) return e;
+    }
+    if (dw)
+        if (int e = check_dense_operand(x, ldx, M, K)) return e;
+    if (dx) {
+        if (int e = check_dense_operand(w, ldw, N, K)) return e;
+        if (int e = check_dense_rows(dx, lddx, M, K, true)) return e;
+    }
+    if (!workspace || (act != pai::ACT_NONE && !saved)) return PAI_ERR_NULL_POINTER;
+    if ((saved && !aligned(saved, 16)) || !aligned(workspace, 256) || !aligned(dw, 2) || !aligned(db, bias_fp32 ? 4 : 2)) return PAI_ERR_MISALIGNED;
+    if (workspace_bytes < pai_dense_bwd_workspace_bytes(M, N, 0)) return PAI_ERR_WORKSPACE_TOO_SMALL;
+    if (int e = require_sm100()) return e;
+    int sms = 0;
+    if (int e = current_device_sms(&sms)) return e;
+    const pai::DenseOperand ws[2] = {{w, ldw}, {nullptr, 0}};
+    void *const dws[2] = {dw, nullptr};
+    void *const dbs[2] = {db, nullptr};
+    return pai::dense_backward({dy, lddy}, {x, ldx}, ws, saved, dx, lddx, dws, dbs, bias_fp32 != 0, workspace, M, N, K, act, dtype == PAI_FP16, sms,
+                               (cudaStream_t)stream);
+}
+
+int pai_gated_bwd(const void *dh, int64_t lddh, const void *x, int64_t ldx, const void *w_gate, int64_t ldwg, const void *w_up, int64_t ldwu,
+                  const void *saved, void *dx, int64_t lddx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, int bias_fp32, void *workspace,
+                  size_t workspace_bytes, long long M, int N, int K, int act, int dtype, void *stream) {
+    if (int e = check_dense_sizes(M, N, K, act, dtype)) return e;
+    if (M < 1) return PAI_ERR_BAD_SHAPE;
+    if (int e = check_dense_rows(dh, lddh, M, N, false)) return e;
+    if (dw_gate || dw_up)
+        if (int e = check_dense_operand(x, ldx, M, K)) return e;
+    // (the weights' addresses also say that the product is gated, so both are wanted whatever is asked for)
+    if (int e = check_dense_operand(w_gate, ldwg, N, K)) return e;
+    if (int e = check_dense_operand(w_up, ldwu, N, K)) return e;
+    if (dx)
+        if (int e = check_dense_rows(dx, lddx, M, K, true)) return e;
+    if (!workspace || !saved) return PAI_ERR_NULL_POINTER;
+    const size_t ba = bias_fp32 ? 4 : 2;
+    if (!aligned(saved, 16) || !aligned(workspace, 256) || !aligned(dw_gate, 2) || !aligned(dw_up, 2) || !aligned(db_gate, ba) || !aligned(db_up, ba))
+        return PAI_ERR_MISALIGNED;
+    if (workspace_bytes < pai_dense_bwd_workspace_bytes(M, N, 1)) return PAI_ERR_WORKSPACE_TOO_SMALL;
+    if (int e = require_sm100()) return e;
+    int sms = 0;
+    if (int e = current_device_sms(&sms)) return e;
+    const pai::DenseOperand ws[2] = {{w_gate, ldwg}, {w_up, ldwu}};
+    void *const dws[2] = {dw_gate, dw_up};
+    void *const dbs[2] = {db_gate, db_up};
+    return pai::dense_backward({dh, lddh}, {x, ldx}, ws, saved, dx, lddx, dws, dbs, bias_fp32 != 0, workspace, M, N, K, act, dtype == PAI_FP16, sms,
+                               (cudaStream_t)stream);
+}
+
+int pai_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld_dst, long long rows, int cols, void *stream) {
+    if (rows < 0 || rows > PAI_DENSE_MAX_ROWS || cols < 1 || cols > PAI_DENSE_MAX_WIDTH) return PAI_ERR_BAD_SHAPE;
+    if (int e = check_dense_rows(src, ld_src, rows, cols, false)) return e;
+    if (!dst) return PAI_ERR_NULL_POINTER;
+    if (ld_dst < pai::dense_ld16(cols)) return PAI_ERR_BAD_SHAPE;
+    if (!aligned(dst, 16) || (ld_dst & 7) != 0) return PAI_ERR_MISALIGNED;
+    if (int e = require_sm100()) return e;
+    if (rows == 0) return PAI_OK;
+    int sms = 0;
+    if (int e = current_device_sms(&sms)) return e;
+    return pai::dense_copy_rows(src, ld_src, dst, ld_dst, rows, cols, sms, (cudaStream_t)stream);
 }
 
 int pai_knn_neighbors(const float *ca, const uint8_t *valid, int64_t *idx, uint8_t *edge_mask, int Z, int N, int K, float max_dist,

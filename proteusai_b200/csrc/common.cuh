@@ -52,6 +52,13 @@ __device__ __forceinline__ void sfu_sincos(float x, float &s, float &c) {
     asm("cos.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(x));
 }
 
+// 2^x on the SFU
+__device__ __forceinline__ float ex2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // sin and cos of 2 pi t for a packed pair of phases t given in REVOLUTIONS, entirely on the FMA pipe:
 // subtract the nearest integer exactly (magic-number rounding), then even/odd polynomials in the
 // fraction f in [-0.5, 0.5] (coefficients: Chebyshev fits of sin(2 pi f)/f and cos(2 pi f) in f^2;

@@ -1,0 +1,234 @@
+// Host side of the feed-forward products: tensor maps, the choice of tile and split, the launches.
+#pragma once
+#include "dense_tile.cuh"
+
+namespace pai {
+
+inline long long dense_ld16(long long cols) { return (cols + 7) / 8 * 8; }  // row pitch of a 16-bit workspace matrix
+
+// Map of a [rows, inner] matrix of 16-bit elements with row pitch `ld` elements, boxes of 64 x box_rows; outside reads as 0.
+static int make_map_16(CUtensorMap *map, const void *base, long long inner, long long rows, long long ld, int box_rows, int half) {
+    EncodeTiledFn enc = get_encode_tiled();
+    if (!enc) return (int)PAI_ERR_UNSUPPORTED;
+    cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+    cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld : dense_ld16(inner)) * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box,
+                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? 0 : (int)PAI_ERR_UNSUPPORTED;
+}
+
+struct DenseOperand {       // a matrix of 16-bit elements
+    const void *p;
+    long long ld;
+};
+
+// One product: out[t, f] (+ epilogue); `a[i]`, `b[i]` the operand pairs, `dual` / `segs` / `groups` as in dense_tile.cuh.
+struct DenseProduct {
+    DenseOperand a[2], b[2];
+    int a_mn, b_mn, dual, segs, groups;
+    long long F, T, R;
+    void *out[2];
+    long long ld_out;
+    const void *bias[2];
+    int bias_fp32;
+    const void *residual;
+    long long ld_res;
+    float *save[2];
+    int act, half;
+};
+
+// Tile height (rows t per CTA) and split of the reduction: the pair with the lowest estimated time.  A CTA's 64-wide reduction block costs
+// the larger of its MMAs (2 tn cycles per accumulator) and its loads (the SM takes about 48 bytes a cycle from L2); CTAs beyond one per SM
+// queue up; a split adds the exchange of partial tiles.
+static void dense_tile_choose(const DenseProduct &d, int sms, int *tn_out, int *splits_out) {
+    const long long kb = (d.R + DT_BK - 1) / DT_BK * d.segs;
+    const int acc = d.dual ? 2 : 1;
+    double best = 1e300;
+    *tn_out = 64, *splits_out = 1;
+    for (int tn = d.b_mn ? 64 : 16; tn <= (d.dual ? 128 : 256); tn *= 2) {
+        if (tn > (d.b_mn ? 64 : 16) && tn / 2 >= d.T) break;
+        const long long tiles = (d.F + DT_FT - 1) / DT_FT * ((d.T + tn - 1) / tn) * d.groups;
+        for (int splits = 1; splits <= 8 && splits <= kb; splits *= 2) {
+            const double rounds = (double)((tiles * splits + sms - 1) / sms);
+            const double mma = 2.0 * tn * acc, load = (128.0 * acc + tn) * 128.0 / 48.0;
+            const double work = (double)((kb + splits - 1) / splits) * (mma > load ? mma : load);
+            const double epi = (splits > 1 ? 1500.0 + tn * acc * 8.0 + (double)tn / splits * 20.0 * acc : tn * 12.0 * acc);
+            const double t = rounds * (work + epi) + 2500.0;
+            if (t < best) best = t, *tn_out = tn, *splits_out = splits;
+        }
+    }
+}
+
+template <bool DUAL>
+static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams &p, long long ctas, int smem, cudaStream_t st) {
+    static bool attr_done[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(dense_tile_kernel<DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        if (e != cudaSuccess) return (int)e;
+        if (dev >= 0 && dev < 64) attr_done[dev] = true;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.blockDim = dim3(DT_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)p.splits;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, dense_tile_kernel<DUAL>, m[0], m[1], m[2], m[3], p);
+}
+
+static int dense_tile_launch(const DenseProduct &d, int sms, cudaStream_t st) {
+    int tn, splits;
+    dense_tile_choose(d, sms, &tn, &splits);
+    DenseTileParams p = {};
+    p.out0 = d.out[0], p.out1 = d.out[1];
+    p.bias0 = d.bias[0], p.bias1 = d.bias[1];
+    p.residual = (const unsigned short *)d.residual;
+    p.save0 = d.save[0], p.save1 = d.save[1];
+    p.ld_out = d.ld_out, p.ld_res = d.ld_res;
+    p.F = (int)d.F, p.T = (int)d.T;
+    p.f_tiles = (int)((d.F + DT_FT - 1) / DT_FT), p.t_tiles = (int)((d.T + tn - 1) / tn);
+    p.splits = splits, p.tn = tn;
+    p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
+    p.a_mn = d.a_mn, p.b_mn = d.b_mn;
+    p.act = d.act, p.half = d.half, p.bias_fp32 = d.bias_fp32;
+    p.idesc = (umma_idesc_bf16(128, tn, d.a_mn != 0, d.b_mn != 0) & ~((7u << 7) | (7u << 10))) | (d.half ? 0u : (1u << 7) | (1u << 10));
+    const long long ctas = (long long)p.f_tiles * p.t_tiles * d.groups * splits;
+    if (ctas > 0x7fffffffll) return (int)PAI_ERR_BAD_SHAPE;
+    const int stage = (d.dual ? 2 : 1) * DT_FT * 128 + tn * 128, kb_cta = (p.kb_total + splits - 1) / splits;
+    int stages = (ctas > sms ? 108 * 1024 : 208 * 1024) / stage;
+    stages = stages > DT_MAX_STAGES ? DT_MAX_STAGES : stages;
+    stages = stages > kb_cta ? kb_cta : stages;
+    p.stages = stages;
+    int smem = stages * stage;
+    const int red = splits > 1 ? tn * DT_FT * 4 * (d.dual ? 2 : 1) : 0;
+    smem = (smem > red ? smem : red) + 1024;
+    CUtensorMap m[4];
+    for (int i = 0; i < 2; ++i) {
+        const DenseOperand &a = d.a[i].p ? d.a[i] : d.a[0], &b = d.b[i].p ? d.b[i] : d.b[0];
+        if (i == 1 && !d.a[1].p) m[1] = m[0];
+        else if (int e = d.a_mn ? make_map_16(&m[i], a.p, d.F, d.R, a.ld, 64, d.half) : make_map_16(&m[i], a.p, d.R, d.F, a.ld, DT_FT, d.half)) return e;
+        if (i == 1 && !d.b[1].p) m[3] = m[2];
+        else if (int e = d.b_mn ? make_map_16(&m[2 + i], b.p, d.T, d.R, b.ld, 64, d.half) : make_map_16(&m[2 + i], b.p, d.R, d.T, b.ld, tn, d.half)) return e;
+    }
+    return d.dual ? dense_tile_launch_as<true>(m, p, ctas, smem, st) : dense_tile_launch_as<false>(m, p, ctas, smem, st);
+}
+
+// ---- the two operators ----------------------------------------------------------------------------------------------
+static int dense_forward(const DenseOperand &x, const DenseOperand (&w)[2], const void *const (&bias)[2], int bias_fp32, const DenseOperand &residual,
+                         void *y, long long ldy, void *saved, long long M, int N, int K, int act, int half, int sms, cudaStream_t st) {
+    DenseProduct d = {};
+    const bool gated = w[1].p != nullptr;
+    d.a[0] = w[0], d.a[1] = w[1];
+    d.b[0] = x;
+    d.dual = gated, d.segs = 1, d.groups = 1;
+    d.F = N, d.T = M, d.R = K;
+    d.out[0] = y, d.ld_out = ldy;
+    d.bias[0] = bias[0], d.bias[1] = bias[1], d.bias_fp32 = bias_fp32;
+    d.residual = residual.p, d.ld_res = residual.ld;
+    d.save[0] = (float *)saved;
+    d.save[1] = saved && gated ? (float *)((char *)saved + saved_bytes_f32(M, N)) : nullptr;
+    d.act = act, d.half = half;
+    return dense_tile_launch(d, sms, st);
+}
+
+// Strips of the elementwise pass: about four CTAs of 256 threads per SM, at least 64 rows each.
+inline int dense_strip_rows(long long M, int N) {
+    const long long col_ctas = (N + 255) / 256, want = 592 / col_ctas > 0 ? 592 / col_ctas : 1;
+    long long strip = (M + want - 1) / want;
+    strip = strip < 64 ? 64 : (strip + 7) / 8 * 8;
+    return (int)strip;
+}
+inline long long dense_strips(long long M, int N) {
+    const int s = dense_strip_rows(M, N);
+    return (M + s - 1) / s;
+}
+inline size_t align256(size_t b) { return (b + 255) / 256 * 256; }
+// workspace: the 16-bit gradient(s) of the pre-activations, then the strips' column sums
+inline size_t dense_d_bytes(long long M, int N) { return align256((size_t)M * dense_ld16(N) * 2); }
+inline size_t dense_bwd_workspace(long long M, int N, int mats) {
+    return mats * (dense_d_bytes(M, N) + align256((size_t)dense_strips(M, N) * N * 4));
+}
+
+static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const DenseOperand (&w)[2], const void *saved, void *dx, long long lddx,
+                          void *const (&dw)[2], void *const (&db)[2], int bias_fp32, void *workspace, long long M, int N, int K, int act, int half,
+                          int sms, cudaStream_t st) {
+    const bool gated = w[1].p != nullptr;
+    const int mats = gated ? 2 : 1;
+    const bool elementwise = gated || act != ACT_NONE;
+    const bool products = dx || dw[0] || dw[1];
+    DenseOperand dz[2] = {dy, {nullptr, 0}};
+    char *ws = (char *)workspace;
+    const long long strips = dense_strips(M, N);
+    DenseBwdElemParams p = {};
+    p.dy = (const unsigned short *)dy.p, p.ld_dy = dy.ld;
+    p.vec_dy = ((uintptr_t)dy.p & 15) == 0 && (dy.ld & 7) == 0;
+    p.M = M, p.N = N, p.act = act, p.half = half, p.strip = dense_strip_rows(M, N);
+    if (elementwise) {
+        p.save0 = (const float *)saved;
+        p.save1 = gated ? (const float *)((const char *)saved + saved_bytes_f32(M, N)) : nullptr;
+        if (products) {
+            p.ld_d = dense_ld16(N);
+            p.d0 = (unsigned short *)ws;
+            p.d1 = gated ? (unsigned short *)(ws + dense_d_bytes(M, N)) : nullptr;
+            dz[0] = {p.d0, p.ld_d}, dz[1] = {p.d1, p.ld_d};
+        }
+    }
+    if (db[0] || db[1]) {
+        p.part0 = (float *)(ws + mats * dense_d_bytes(M, N));
+        p.part1 = gated ? p.part0 + align256((size_t)strips * N * 4) / 4 : nullptr;
+    }
+    if ((elementwise && products) || p.part0) {
+        const dim3 grid((N + 255) / 256, (unsigned)strips);
+        if (gated) dense_bwd_elem_kernel<true><<<grid, 256, 0, st>>>(p);
+        else dense_bwd_elem_kernel<false><<<grid, 256, 0, st>>>(p);
+        if (int e = (int)cudaPeekAtLastError()) return e;
+    }
+    if (p.part0) {
+        // (one of two bias gradients alone: its own sums go into the grid's first row)
+        const float *first = db[0] ? p.part0 : p.part1;
+        void *out = db[0] ? db[0] : db[1];
+        const dim3 grid((N + 31) / 32, db[0] && db[1] ? 2 : 1);
+        dense_colsum_kernel<<<grid, 256, 0, st>>>(first, p.part1, out, db[1], N, (int)strips, half, bias_fp32);
+        if (int e = (int)cudaPeekAtLastError()) return e;
+    }
+    if (dx) {
+        DenseProduct d = {};
+        d.a[0] = w[0], d.a[1] = w[1], d.a_mn = 1;
+        d.b[0] = dz[0], d.b[1] = dz[1];
+        d.segs = mats, d.groups = 1;
+        d.F = K, d.T = M, d.R = N;
+        d.out[0] = dx, d.ld_out = lddx, d.half = half;
+        if (int e = dense_tile_launch(d, sms, st)) return e;
+    }
+    if (dw[0] || dw[1]) {
+        DenseProduct d = {};
+        d.a[0] = x, d.a_mn = 1, d.b_mn = 1;
+        d.segs = 1, d.groups = dw[0] && dw[1] ? 2 : 1;
+        d.b[0] = dw[0] ? dz[0] : dz[1], d.out[0] = dw[0] ? dw[0] : dw[1];
+        if (d.groups == 2) d.b[1] = dz[1], d.out[1] = dw[1];
+        d.F = K, d.T = N, d.R = M;
+        d.ld_out = K, d.half = half;
+        if (int e = dense_tile_launch(d, sms, st)) return e;
+    }
+    return 0;
+}
+
+static int dense_copy_rows(const void *src, long long ld_src, void *dst, long long ld_dst, long long rows, int cols, int sms, cudaStream_t st) {
+    const long long n = rows * ((cols + 7) / 8);
+    long long blocks = (n + 255) / 256;
+    if (blocks > (long long)sms * 32) blocks = (long long)sms * 32;
+    dense_copy_rows_kernel<<<(unsigned)blocks, 256, 0, st>>>((const unsigned short *)src, ld_src, (unsigned short *)dst, ld_dst, rows, cols);
+    return (int)cudaPeekAtLastError();
+}
+
+}  // namespace pai

@@ -1,0 +1,276 @@
+// Shared parts of the feed-forward products (dense_tile.cuh): activations and their derivatives, the layout of the
+// saved pre-activations, the elementwise half of the backward pass, and the copy that aligns an operand's rows.
+//
+//   linear   y = act(z) + r,  z = x W^T + b             dz = dy act'(z)
+//   gated    h = act(g) u,    g = x Wg^T + bg, u = ...   dg = dh u act'(g), du = dh act(g)
+//
+// Inputs and outputs are bf16 or fp16; products accumulate in fp32 and everything up to the one rounding of each output is fp32.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+
+namespace pai {
+
+enum { ACT_NONE = 0, ACT_GELU = 1, ACT_SILU = 2, ACT_RELU = 3, ACT_SIGMOID = 4, ACT_COUNT = 5 };
+
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// log2 Phi(-a), a >= 0, as a polynomial of degree 7: Chebyshev fit of log2 of the normal distribution function on [0, 6], so that
+// 2^p has a RELATIVE error below 4e-6 there (half a bf16 step is 2^-9 .. 2^-8, half an fp16 step 2^-12 .. 2^-11).  Beyond 6 it keeps
+// falling (its leading coefficient is negative), where x Phi(x) is below 1e-8 in magnitude: the absolute error of x Phi(x) stays
+// below 6e-7 on the whole negative axis.  One SFU operation, against two for the rational form of erfc.
+#define PAI_PHI_COEFFS                                                                                                    \
+    {-9.999943403e-01f, -1.151269147e+00f, -4.584097768e-01f, -5.402068712e-02f, 8.539461332e-03f, -9.388679333e-04f, \
+     6.268140101e-05f,  -1.889626234e-06f}
+
+__device__ __forceinline__ float normal_cdf(float x) {
+    constexpr float c[8] = PAI_PHI_COEFFS;
+    const float a = fabsf(x);
+    float p = c[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = fmaf(p, a, c[i]);
+    const float e = ex2_approx(p);
+    return x < 0.f ? e : 1.f - e;
+}
+// the same for a pair, the polynomial in packed arithmetic
+__device__ __forceinline__ void normal_cdf2(float x0, float x1, float &phi0, float &phi1) {
+    constexpr float c[8] = PAI_PHI_COEFFS;
+    const f2_t a = f2_pack(fabsf(x0), fabsf(x1));
+    f2_t p = f2_pack(c[7], c[7]);
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = f2_fma(p, a, f2_pack(c[i], c[i]));
+    float p0, p1;
+    f2_unpack(p, p0, p1);
+    const float e0 = ex2_approx(p0), e1 = ex2_approx(p1);
+    phi0 = x0 < 0.f ? e0 : 1.f - e0;
+    phi1 = x1 < 0.f ? e1 : 1.f - e1;
+}
+__device__ __forceinline__ float sigmoid_f(float x) { return rcp_approx(1.f + ex2_approx(-1.4426950408889634f * x)); }
+
+template <int ACT>
+__device__ __forceinline__ void act_pair(float &a, float &b) {
+    if (ACT == ACT_GELU) {
+        float pa, pb;
+        normal_cdf2(a, b, pa, pb);
+        a *= pa, b *= pb;
+    } else if (ACT == ACT_SILU) {
+        a *= sigmoid_f(a), b *= sigmoid_f(b);
+    } else if (ACT == ACT_RELU) {
+        a = a < 0.f ? 0.f : a, b = b < 0.f ? 0.f : b;  // (a NaN stays one)
+    } else if (ACT == ACT_SIGMOID) {
+        a = sigmoid_f(a), b = sigmoid_f(b);
+    }
+}
+
+// act(z) and act'(z)
+__device__ __forceinline__ void act_and_slope(int act, float z, float &a, float &d) {
+    switch (act) {
+        case ACT_GELU: {
+            const float phi = normal_cdf(z);
+            a = z * phi;
+            d = fmaf(z * 0.3989422804014327f, ex2_approx(-0.7213475204444817f * z * z), phi);
+            break;
+        }
+        case ACT_SILU: {
+            const float s = sigmoid_f(z);
+            a = z * s;
+            d = s * fmaf(z, 1.f - s, 1.f);
+            break;
+        }
+        case ACT_RELU:
+            a = z < 0.f ? 0.f : z;
+            d = z > 0.f ? 1.f : 0.f;
+            break;
+        case ACT_SIGMOID:
+            a = sigmoid_f(z);
+            d = a * (1.f - a);
+            break;
+        default: a = z, d = 1.f;
+    }
+}
+
+// ---- 16-bit types: `half` != 0 is fp16, 0 is bf16 -----------------------------------------------------------------
+__device__ __forceinline__ unsigned short to_bits16(float v, int half) {
+    return half ? __half_as_ushort(__float2half_rn(v)) : __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+__device__ __forceinline__ float from_bits16(unsigned short b, int half) {
+    return half ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
+}
+__device__ __forceinline__ uint32_t pack_bits16(float lo, float hi, int half) {
+    if (half) {
+        const __half2 h = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&b);
+}
+__device__ __forceinline__ void unpack_bits16(uint32_t w, int half, float &lo, float &hi) {
+    if (half) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w));
+        lo = f.x, hi = f.y;
+    } else {
+        lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xffff0000u);
+    }
+}
+
+// ---- saved pre-activations ----------------------------------------------------------------------------------------
+// What the backward pass needs besides its inputs is z (linear, with an activation) or g and u (gated).  Rounding them to the
+// tensors' own 16-bit type would add an error as large as the outputs' rounding; they are kept in fp32, in blocks of 32 rows x 32
+// columns laid out [piece of 4 columns][row][4]: both a thread per row and a thread per column write whole sectors.
+__host__ __device__ inline size_t saved_blocks(long long rows, int cols) { return (size_t)((rows + 31) / 32) * (size_t)((cols + 31) / 32); }
+__host__ __device__ inline size_t saved_bytes_f32(long long rows, int cols) { return saved_blocks(rows, cols) * 4096; }
+__device__ __forceinline__ size_t saved_index_f32(long long row, int col, int col_blocks) {
+    return (((size_t)(row >> 5) * col_blocks + (col >> 5)) * 8 + ((col & 31) >> 2)) * 128 + (size_t)(row & 31) * 4 + (col & 3);
+}
+
+// ---- elementwise half of the backward pass ------------------------------------------------------------------------
+// One warp covers 8 rows x 32 columns a step (4 lanes x 8 columns per row), a CTA 8 rows x 256 columns; it walks down a strip of
+// `strip` rows and keeps the column sums of what it writes in registers (the bias gradients), joined over the eight row lanes by
+// shuffles and written as one partial row per strip; dense_colsum_kernel adds the strips in order, so the sums are reproducible.
+// HBM-bound: linear reads dy (2 B) and z (4 B) and writes dz (2 B) per element.
+struct DenseBwdElemParams {
+    const unsigned short *dy;
+    long long ld_dy;
+    const float *save0, *save1;     // z, or g and u
+    unsigned short *d0, *d1;        // dz, or dg and du; NULL: not wanted (d0: sums of dy alone)
+    long long ld_d;
+    float *part0, *part1;           // [strips, N] column sums, or NULL
+    long long M;
+    int N, act, half, strip, vec_dy;
+};
+
+template <bool DUAL>
+__global__ void __launch_bounds__(256) dense_bwd_elem_kernel(const __grid_constant__ DenseBwdElemParams p) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c0 = blockIdx.x * 256 + warp * 32 + (lane & 3) * 8;
+    const long long r_begin = (long long)blockIdx.y * p.strip;
+    const long long r_end = r_begin + p.strip < p.M ? r_begin + p.strip : p.M;
+    const int col_blocks = (p.N + 31) >> 5;
+    float s0[8], s1[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s0[i] = s1[i] = 0.f;
+    const int nc = p.N - c0;  // columns of this thread that exist (may be <= 0 or > 8)
+    if (nc > 0) {
+        for (long long r = r_begin + (lane >> 2); r < r_end; r += 8) {
+            float dy[8];
+            const unsigned short *src = p.dy + r * p.ld_dy + c0;
+            if (p.vec_dy && nc >= 8) {
+                const uint4 v = *reinterpret_cast<const uint4 *>(src);
+                unpack_bits16(v.x, p.half, dy[0], dy[1]);
+                unpack_bits16(v.y, p.half, dy[2], dy[3]);
+                unpack_bits16(v.z, p.half, dy[4], dy[5]);
+                unpack_bits16(v.w, p.half, dy[6], dy[7]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) dy[i] = i < nc ? from_bits16(src[i], p.half) : 0.f;
+            }
+            float o0[8], o1[8];
+            if (p.save0) {
+                const size_t at = saved_index_f32(r, c0, col_blocks);
+                const float4 za = *reinterpret_cast<const float4 *>(p.save0 + at), zb = *reinterpret_cast<const float4 *>(p.save0 + at + 128);
+                const float z[8] = {za.x, za.y, za.z, za.w, zb.x, zb.y, zb.z, zb.w};
+                if (DUAL) {
+                    const float4 ua = *reinterpret_cast<const float4 *>(p.save1 + at), ub = *reinterpret_cast<const float4 *>(p.save1 + at + 128);
+                    const float u[8] = {ua.x, ua.y, ua.z, ua.w, ub.x, ub.y, ub.z, ub.w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float a, d;
+                        act_and_slope(p.act, z[i], a, d);
+                        o0[i] = dy[i] * u[i] * d;
+                        o1[i] = dy[i] * a;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        float a, d;
+                        act_and_slope(p.act, z[i], a, d);
+                        o0[i] = dy[i] * d;
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) o0[i] = dy[i];
+            }
+            // (columns past N: dy is 0 there but z is not defined; they are never written and their sums never stored)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s0[i] += o0[i];
+                if (DUAL) s1[i] += o1[i];
+            }
+            if (p.d0) {  // rows of d0 / d1 are padded to a multiple of 8 columns: whole 16-byte words, the tail is never read
+                *reinterpret_cast<uint4 *>(p.d0 + r * p.ld_d + c0) = make_uint4(pack_bits16(o0[0], o0[1], p.half), pack_bits16(o0[2], o0[3], p.half),
+                                                                               pack_bits16(o0[4], o0[5], p.half), pack_bits16(o0[6], o0[7], p.half));
+                if (DUAL)
+                    *reinterpret_cast<uint4 *>(p.d1 + r * p.ld_d + c0) =
+                        make_uint4(pack_bits16(o1[0], o1[1], p.half), pack_bits16(o1[2], o1[3], p.half), pack_bits16(o1[4], o1[5], p.half),
+                                   pack_bits16(o1[6], o1[7], p.half));
+            }
+        }
+    }
+    if (p.part0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                s0[i] += __shfl_xor_sync(0xffffffffu, s0[i], o);
+                if (DUAL) s1[i] += __shfl_xor_sync(0xffffffffu, s1[i], o);
+            }
+        }
+        if (lane < 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < nc) {
+                    p.part0[(size_t)blockIdx.y * p.N + c0 + i] = s0[i];
+                    if (DUAL && p.part1) p.part1[(size_t)blockIdx.y * p.N + c0 + i] = s1[i];
+                }
+        }
+    }
+}
+
+// out[c] = sum over strips of part[s, c], in order of s
+__global__ void __launch_bounds__(256) dense_colsum_kernel(const float *__restrict__ part0, const float *__restrict__ part1, void *out0, void *out1,
+                                                           int N, int strips, int half, int out_fp32) {
+    const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+    const float *part = blockIdx.y ? part1 : part0;
+    void *out = blockIdx.y ? out1 : out0;
+    __shared__ float sm[8][32];
+    float s = 0.f;
+    if (c < N)
+        for (int i = w; i < strips; i += 8) s += part[(size_t)i * N + c];
+    sm[w][threadIdx.x & 31] = s;
+    __syncthreads();
+    if (w == 0 && c < N) {
+        for (int i = 1; i < 8; ++i) s += sm[i][threadIdx.x];
+        if (out_fp32) reinterpret_cast<float *>(out)[c] = s;
+        else reinterpret_cast<unsigned short *>(out)[c] = to_bits16(s, half);
+    }
+}
+
+// dst[r, 0 .. cols) = src[r, 0 .. cols) for rows of any alignment: TMA wants 16-byte aligned rows
+__global__ void __launch_bounds__(256) dense_copy_rows_kernel(const unsigned short *__restrict__ src, long long ld_src, unsigned short *__restrict__ dst,
+                                                              long long ld_dst, long long rows, int cols) {
+    const int words = (cols + 7) >> 3;
+    const long long n = rows * words, stride = (long long)gridDim.x * 256;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
+        const long long r = i / words;
+        const int c = (int)(i - r * words) * 8;
+        const unsigned short *s = src + r * ld_src + c;
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t lo = c + 2 * k < cols ? s[2 * k] : 0, hi = c + 2 * k + 1 < cols ? s[2 * k + 1] : 0;
+            w[k] = lo | hi << 16;
+        }
+        *reinterpret_cast<uint4 *>(dst + r * ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+}  // namespace pai

@@ -1,0 +1,270 @@
+// dense_tile_kernel: out[t, f] = epilogue( sum_r A[f, r] B[t, r] ) on the tensor cores, one output tile of 128 f x tn t per CTA, the
+// reduction split over a cluster where there are too few tiles to fill the GPU.
+//
+// The contiguous axis of the output (f) is the M axis of the MMA, so an accumulator lane is an output column: the 32 lanes of a warp store
+// 64 contiguous bytes of a row, a bias is one register per thread, and a single token costs an MMA of N = 16 rather than 128 rows of
+// which one is wanted.  The same kernel runs every product of the two operators:
+//     forward   f = output feature, t = token,           r = input feature:   A = W        (K-major),  B = x  (K-major)
+//     dx        f = input feature,  t = token,           r = output feature:  A = W        (MN-major), B = dz (K-major)
+//     dW        f = input feature,  t = output feature,  r = token:           A = x        (MN-major), B = dz (MN-major)
+// Gated forward: two A operands (Wg, Wu) against one B into two accumulators (DUAL).  Gated dx: two pairs of operands in sequence into one
+// accumulator (kb_seg).  Gated dW: two output groups (the second with its own B and output).
+//
+// Split reduction: the CTAs of a cluster each take a run of the 64-wide reduction blocks, put their partial tile into their own shared
+// memory and then each finish tn / splits of the rows, adding the partials of all ranks in rank order through distributed shared memory:
+// one launch, no workspace, no atomics, the same bits every time.
+//
+// Tensor memory is given back before the cluster barrier: a CTA that waits for another never holds columns that the other may need.
+#pragma once
+#include "dense_ops.cuh"
+#include "tc.cuh"
+
+namespace pai {
+
+constexpr int DT_THREADS = 256;
+constexpr int DT_FT = 128;        // output columns (MMA rows) per tile
+constexpr int DT_BK = 64;         // reduction block: 128 bytes, one swizzle row
+constexpr int DT_MAX_STAGES = 8;
+
+struct DenseTileParams {
+    void *out0, *out1;              // 16-bit outputs of the groups
+    const void *bias0, *bias1;      // [F] of the accumulators (DUAL: both), or NULL
+    const unsigned short *residual; // [T, F], or NULL
+    float *save0, *save1;           // saved pre-activations (saved_index_f32), or NULL
+    long long ld_out, ld_res;
+    int F, T;
+    int f_tiles, t_tiles, splits, tn, stages;
+    int kb_seg, kb_total;           // 64-wide reduction blocks of the first operand pair, of both
+    int a_mn, b_mn;                 // operands stored with the reduction as their slow axis
+    int act, half, bias_fp32;
+    uint32_t idesc;
+};
+
+__device__ __forceinline__ void tma_load_2d(void *dst_smem, const CUtensorMap *map, int c0, int c1, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(smem_u32(dst_smem)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
+        : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+                 : "=f"(v)
+                 : "r"(addr), "r"(rank)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ float load_bias(const void *b, int i, int fp32, int half) {
+    return fp32 ? reinterpret_cast<const float *>(b)[i] : from_bits16(reinterpret_cast<const unsigned short *>(b)[i], half);
+}
+
+// One value of the output from its accumulator(s): column f (bias in b0, b1), row t.
+template <bool DUAL, int ACT>
+__device__ __forceinline__ float dense_finish(const DenseTileParams &p, float v0, float v1, float b0, float b1, int f, int t, int col_blocks) {
+    v0 += b0;
+    if (DUAL) v1 += b1;
+    if (p.save0) {
+        const size_t at = saved_index_f32(t, f, col_blocks);
+        p.save0[at] = v0;
+        if (DUAL) p.save1[at] = v1;
+    }
+    float dummy = 0.f;
+    act_pair<ACT>(v0, dummy);
+    return DUAL ? v0 * v1 : v0;
+}
+
+template <bool DUAL, int ACT>
+__device__ __forceinline__ void dense_epilogue(const DenseTileParams &p, uint32_t tmem, float *red, int f0, int t0, int group, int rank) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    unsigned short *out = reinterpret_cast<unsigned short *>(group ? p.out1 : p.out0);
+    const int col_blocks = (p.F + 31) >> 5;
+    if (p.splits == 1) {
+        const int q = warp & 3, f = f0 + q * 32 + lane;
+        const bool live = f < p.F;
+        const float b0 = live && p.bias0 ? load_bias(p.bias0, f, p.bias_fp32, p.half) : 0.f;
+        const float b1 = DUAL && live && p.bias1 ? load_bias(p.bias1, f, p.bias_fp32, p.half) : 0.f;
+        for (int c = (warp >> 2) * 16; c < p.tn; c += 32) {
+            if (t0 + c >= p.T) break;  // (warp-uniform)
+            uint32_t v[16], u[16];
+            tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+            if (DUAL) tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + p.tn + c, u);
+            float r[16];
+            const int nt = p.T - t0 - c;
+            if (p.residual) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) r[j] = (live && j < nt) ? from_bits16(p.residual[(long long)(t0 + c + j) * p.ld_res + f], p.half) : 0.f;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) r[j] = 0.f;
+            }
+            tmem_wait_ld();
+            if (live) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    if (j < nt) {
+                        const int t = t0 + c + j;
+                        const float y = dense_finish<DUAL, ACT>(p, __uint_as_float(v[j]), DUAL ? __uint_as_float(u[j]) : 0.f, b0, b1, f, t, col_blocks);
+                        out[(long long)t * p.ld_out + f] = to_bits16(y + r[j], p.half);
+                    }
+            }
+        }
+        return;
+    }
+    // the cluster's partial tiles: rows [rank, rank + 1) tn / splits of the tile are this CTA's to finish
+    const int fl = tid & 127, f = f0 + fl;
+    if (f >= p.F) return;
+    const float b0 = p.bias0 ? load_bias(p.bias0, f, p.bias_fp32, p.half) : 0.f;
+    const float b1 = DUAL && p.bias1 ? load_bias(p.bias1, f, p.bias_fp32, p.half) : 0.f;
+    const int rows = p.tn / p.splits;
+    for (int j = tid >> 7; j < rows; j += 2) {
+        const int tl = rank * rows + j, t = t0 + tl;
+        if (t >= p.T) break;
+        float v0 = 0.f, v1 = 0.f;
+        const uint32_t at = smem_u32(red + (size_t)tl * DT_FT + fl);
+        for (int s = 0; s < p.splits; ++s) {
+            v0 += ld_cluster_f32(at, s);
+            if (DUAL) v1 += ld_cluster_f32(at + (uint32_t)p.tn * DT_FT * 4, s);
+        }
+        float y = dense_finish<DUAL, ACT>(p, v0, v1, b0, b1, f, t, col_blocks);
+        if (p.residual) y += from_bits16(p.residual[(long long)t * p.ld_res + f], p.half);
+        out[(long long)t * p.ld_out + f] = to_bits16(y, p.half);
+    }
+}
+
+template <bool DUAL>
+__global__ void __launch_bounds__(DT_THREADS) dense_tile_kernel(const __grid_constant__ CUtensorMap ma0, const __grid_constant__ CUtensorMap ma1,
+                                                                const __grid_constant__ CUtensorMap mb0, const __grid_constant__ CUtensorMap mb1,
+                                                                const __grid_constant__ DenseTileParams p) {
+    extern __shared__ uint8_t dt_raw[];
+    __shared__ uint64_t bar_full[DT_MAX_STAGES], bar_free[DT_MAX_STAGES], bar_done;
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag;
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(dt_raw) + 1023) & ~(uintptr_t)1023);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = (int)blockIdx.x % p.splits, tile = (int)blockIdx.x / p.splits;
+    const int f0 = (tile % p.f_tiles) * DT_FT, rest = tile / p.f_tiles;
+    const int t0 = (rest % p.t_tiles) * p.tn, group = rest / p.t_tiles;
+    const int k0 = (int)((long long)p.kb_total * rank / p.splits), k1 = (int)((long long)p.kb_total * (rank + 1) / p.splits);
+    const uint32_t a_bytes = (DUAL ? 2 : 1) * DT_FT * 128, b_bytes = (uint32_t)p.tn * 128;
+    const uint32_t stage_bytes = a_bytes + b_bytes;
+    uint32_t cols = 32;
+    while (cols < (uint32_t)p.tn * (DUAL ? 2 : 1)) cols <<= 1;
+
+    if (warp == 2) tmem_alloc(&tmem_base, cols);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < p.stages; ++i) {
+            mbar_init(&bar_full[i], 1);
+            mbar_init(&bar_free[i], 1);
+        }
+        mbar_init(&bar_done, 1);
+        abort_flag = 0;
+        mbar_fence_init();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+
+    if (warp == 0 && lane == 0) {
+        int slot = 0;
+        uint32_t phase = 0;
+        for (int kb = k0; kb < k1; ++kb) {
+            if (!mbar_wait_abortable(&bar_free[slot], phase ^ 1, &abort_flag)) break;
+            uint8_t *a = base + (size_t)slot * stage_bytes, *b = a + a_bytes;
+            mbar_expect_tx(&bar_full[slot], stage_bytes);
+            const bool second = kb >= p.kb_seg;
+            const int r = (second ? kb - p.kb_seg : kb) * DT_BK;
+            const CUtensorMap *ma = second ? &ma1 : &ma0, *mb = (second || group) ? &mb1 : &mb0;
+            if (p.a_mn) {
+                tma_load_2d(a, ma, f0, r, &bar_full[slot]);
+                tma_load_2d(a + 8192, ma, f0 + 64, r, &bar_full[slot]);
+            } else {
+                tma_load_2d(a, ma, r, f0, &bar_full[slot]);
+                if (DUAL) tma_load_2d(a + 16384, &ma1, r, f0, &bar_full[slot]);
+            }
+            if (p.b_mn) {
+                for (int i = 0; i < p.tn; i += 64) tma_load_2d(b + i * 128, mb, t0 + i, r, &bar_full[slot]);
+            } else {
+                tma_load_2d(b, mb, r, t0, &bar_full[slot]);
+            }
+            if (++slot == p.stages) slot = 0, phase ^= 1;
+        }
+    } else if (warp == 1 && lane == 0) {
+        // K-major: rows of 128 bytes, 8-row groups 1024 apart, 16 elements of the reduction 32 bytes on.
+        // MN-major: 64-wide panels 8192 apart, 8 steps of the reduction 1024 apart, 16 of them 2048 on.
+        const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
+        const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
+        int slot = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int kb = k0; kb < k1; ++kb) {
+            if (!mbar_wait_abortable(&bar_full[slot], phase, &abort_flag)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            const uint32_t a = smem_u32(base) + (uint32_t)slot * stage_bytes;
+            const uint64_t ad = umma_desc_sw128(a, a_lbo, 1024), bd = umma_desc_sw128(a + a_bytes, b_lbo, 1024);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                umma_ss(tmem, ad + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
+                if (DUAL) umma_ss(tmem + p.tn, ad + (16384 >> 4) + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
+            }
+            umma_commit(&bar_free[slot]);
+            if (++slot == p.stages) slot = 0, phase ^= 1;
+        }
+        if (ok) umma_commit(&bar_done);
+    }
+    __syncwarp();
+    const bool ok = mbar_wait_abortable(&bar_done, 0, &abort_flag);
+    tc_fence_after();
+    float *red = reinterpret_cast<float *>(base);
+    if (p.splits > 1) {
+        if (ok) {
+            const int q = warp & 3;
+            for (int c = (warp >> 2) * 16; c < p.tn * (DUAL ? 2 : 1); c += 32) {
+                uint32_t v[16];
+                tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) red[(size_t)(c + j) * DT_FT + q * 32 + lane] = __uint_as_float(v[j]);
+            }
+        }
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 2) {
+            tc_fence_after();
+            tmem_relinquish();
+            tmem_dealloc(tmem, cols);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
+    }
+    if (ok) {
+        switch (p.act) {
+            case ACT_GELU: dense_epilogue<DUAL, ACT_GELU>(p, tmem, red, f0, t0, group, rank); break;
+            case ACT_SILU: dense_epilogue<DUAL, ACT_SILU>(p, tmem, red, f0, t0, group, rank); break;
+            case ACT_RELU: dense_epilogue<DUAL, ACT_RELU>(p, tmem, red, f0, t0, group, rank); break;
+            case ACT_SIGMOID: dense_epilogue<DUAL, ACT_SIGMOID>(p, tmem, red, f0, t0, group, rank); break;
+            default: dense_epilogue<DUAL, ACT_NONE>(p, tmem, red, f0, t0, group, rank);
+        }
+    }
+    __syncwarp();
+    if (p.splits > 1) {
+        cluster_arrive();  // nobody leaves while its partial tile is being read
+        cluster_wait();
+    } else {
+        tc_fence_before();
+        __syncthreads();
+        if (warp == 2) {
+            tc_fence_after();
+            tmem_relinquish();
+            tmem_dealloc(tmem, cols);
+        }
+    }
+}
+
+}  // namespace pai
