@@ -320,9 +320,9 @@ int pai_gelu_bf16(const void *x, void *out, long long n, void *stream);
  * rounded once, and dz (dg, du) once to `dtype` in between.
  * Operands of the products (x and w*; dy of pai_linear_bwd without an activation) need 16-byte aligned rows: base 16-byte aligned, pitch a
  * multiple of 8 elements (pai_copy_rows16 makes such a copy).  y, h, residual, dx, and dy otherwise, may have any alignment and pitch.
- *   saved      NULL (inference), or pai_dense_saved_bytes(M, N, gated) bytes, 16-byte aligned: the pre-activations for the backward call,
+ *   saved      NULL (inference), or pai_dense_saved_bytes(M, N, K, gated, dtype) bytes, 16-byte aligned: the pre-activations for the backward call,
  *              in a layout of the library's own; pai_linear_bwd without an activation needs none.
- *   workspace  pai_dense_bwd_workspace_bytes(M, N, gated) bytes, 256-byte aligned.
+ *   workspace  pai_dense_bwd_workspace_bytes(M, N, K, gated) bytes, 256-byte aligned.
  * Limits: M < 2^31 - 2^16, N and K <= 2^20.  Results are the same bits from call to call.
  *   pai_copy_rows16  dst[r, c] = src[r, c] for rows of 16-bit elements of any alignment into 16-byte aligned rows; columns up to the next
  *                    multiple of 8 are written as zeros.
@@ -331,8 +331,8 @@ enum pai_dtype { PAI_BF16 = 0, PAI_FP16 = 1 };
 enum pai_act { PAI_ACT_NONE = 0, PAI_ACT_GELU = 1 /* erf form */, PAI_ACT_SILU = 2, PAI_ACT_RELU = 3, PAI_ACT_SIGMOID = 4 };
 #define PAI_DENSE_MAX_ROWS 2147418111ll
 #define PAI_DENSE_MAX_WIDTH 1048576
-size_t pai_dense_saved_bytes(long long M, int N, int gated);
-size_t pai_dense_bwd_workspace_bytes(long long M, int N, int gated);
+size_t pai_dense_saved_bytes(long long M, int N, int K, int gated, int dtype);
+size_t pai_dense_bwd_workspace_bytes(long long M, int N, int K, int gated);
 int pai_linear_fwd(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, int bias_fp32, const void *residual, int64_t ldr,
                    void *y, int64_t ldy, void *saved, long long M, int N, int K, int act, int dtype, void *stream);
 int pai_gated_fwd(const void *x, int64_t ldx, const void *w_gate, int64_t ldwg, const void *w_up, int64_t ldwu, const void *bias_gate,
@@ -406,7 +406,11 @@ enum pai_tune_key {
     PAI_TUNE_GA_NO_ORDER = 7,     /* 1: issue the samples in natural order instead of longest first */
     PAI_TUNE_WE_MIXED = 8,        /* 1: separate SFU and polynomial warps (we_fwd_mixed_kernel) instead of both pipes in every warp;
                                      measured 12 % slower at N = 16384, kept for comparison (default 0) */
-    PAI_TUNE_COUNT = 9
+    PAI_TUNE_DENSE_KERNEL = 9,    /* feed-forward products: 1 = dense_tile_kernel, 2 = dense_pair_kernel (set it before the forward call and leave
+                                     it until the backward call has been made: the saved pre-activations go by the kernel) */
+    PAI_TUNE_DENSE_WIDTH = 10,    /* with it: rows of a tile (16 .. 256), accumulator columns of a pair's tile (128, 256) */
+    PAI_TUNE_DENSE_SPLITS = 11,   /* with it: split of the reduction (tile: 1, 2, 4, 8; pair: weight gradients only, 1 .. 16) */
+    PAI_TUNE_COUNT = 12
 };
 int pai_tune_set(int key, int value);
 int pai_selftest_wait_timeout(void *stream);

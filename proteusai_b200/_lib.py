@@ -41,8 +41,8 @@ SIGNATURES = {
                                 c_int, c_int, c_int, c_int, c_void_p]),
     "pai_add_layernorm_bf16": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, ctypes.c_longlong, c_int, c_float, c_void_p]),
     "pai_gelu_bf16": (c_int, [c_void_p, c_void_p, ctypes.c_longlong, c_void_p]),
-    "pai_dense_saved_bytes": (c_size_t, [c_int64, c_int, c_int]),
-    "pai_dense_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int]),
+    "pai_dense_saved_bytes": (c_size_t, [c_int64, c_int, c_int, c_int, c_int]),
+    "pai_dense_bwd_workspace_bytes": (c_size_t, [c_int64, c_int, c_int, c_int]),
     "pai_linear_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
                                c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "pai_gated_fwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_int64, c_void_p,
@@ -63,7 +63,7 @@ SIGNATURES = {
 # enum pai_we_flags / enum pai_tune_key of the header
 WE_REPRODUCIBLE = 1
 TUNE = {"we_ks": 0, "we_tj": 1, "we_waves": 2, "we_range_reduce": 3, "we_poly_pairs": 4, "we_no_tma": 5,
-        "ga_no_far_skip": 6, "ga_no_order": 7, "we_mixed": 8}
+        "ga_no_far_skip": 6, "ga_no_order": 7, "we_mixed": 8, "dense_kernel": 9, "dense_width": 10, "dense_splits": 11}
 TUNE_DEFAULTS = {"we_poly_pairs": 2}
 
 _lib = None

@@ -89,6 +89,7 @@ int g_tune[PAI_TUNE_COUNT] = {
     /* PAI_TUNE_WE_KS */ 0,        /* PAI_TUNE_WE_TJ */ 0,          /* PAI_TUNE_WE_WAVES */ 0,
     /* PAI_TUNE_WE_RANGE_REDUCE */ 0, /* PAI_TUNE_WE_POLY_PAIRS */ 2, /* PAI_TUNE_WE_NO_TMA */ 0,
     /* PAI_TUNE_GA_NO_FAR_SKIP */ 0,  /* PAI_TUNE_GA_NO_ORDER */ 0,   /* PAI_TUNE_WE_MIXED */ 0,
+    /* PAI_TUNE_DENSE_KERNEL */ 0,    /* PAI_TUNE_DENSE_WIDTH */ 0,   /* PAI_TUNE_DENSE_SPLITS */ 0,
 };
 
 // register-only sin+cos loop: 8 independent chains per thread
@@ -638,14 +639,20 @@ int check_dense_rows(const void *p, int64_t ld, long long rows, int cols, bool w
 }
 }  // namespace
 
-size_t pai_dense_saved_bytes(long long M, int N, int gated) {
-    if (M < 1 || M > PAI_DENSE_MAX_ROWS || N < 1 || N > PAI_DENSE_MAX_WIDTH) return 0;
-    return (gated ? 2 : 1) * pai::saved_bytes_f32(M, N);
+// (the sizes go by the kernels that run, which go by the device's number of SMs; without a device, by a B200's)
+static int sms_or_default(void) {
+    int sms = 0;
+    return current_device_sms(&sms) ? 148 : sms;
 }
 
-size_t pai_dense_bwd_workspace_bytes(long long M, int N, int gated) {
-    if (M < 1 || M > PAI_DENSE_MAX_ROWS || N < 1 || N > PAI_DENSE_MAX_WIDTH) return 0;
-    return pai::dense_bwd_workspace(M, N, gated ? 2 : 1);
+size_t pai_dense_saved_bytes(long long M, int N, int K, int gated, int dtype) {
+    if (check_dense_sizes(M, N, K, 0, dtype) || M < 1) return 0;
+    return (gated ? 2 : 1) * pai::dense_saved_matrix(M, N, K, gated != 0, dtype == PAI_FP16, sms_or_default());
+}
+
+size_t pai_dense_bwd_workspace_bytes(long long M, int N, int K, int gated) {
+    if (check_dense_sizes(M, N, K, 0, PAI_BF16) || M < 1) return 0;
+    return pai::dense_bwd_workspace(M, N, K, gated ? 2 : 1, sms_or_default());
 }
 
 int pai_linear_fwd(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias, int bias_fp32, const void *residual, int64_t ldr,
@@ -704,7 +711,7 @@ int pai_linear_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, con
     }
     if (!workspace || (act != pai::ACT_NONE && !saved)) return PAI_ERR_NULL_POINTER;
     if ((saved && !aligned(saved, 16)) || !aligned(workspace, 256) || !aligned(dw, 2) || !aligned(db, bias_fp32 ? 4 : 2)) return PAI_ERR_MISALIGNED;
-    if (workspace_bytes < pai_dense_bwd_workspace_bytes(M, N, 0)) return PAI_ERR_WORKSPACE_TOO_SMALL;
+    if (workspace_bytes < pai_dense_bwd_workspace_bytes(M, N, K, 0)) return PAI_ERR_WORKSPACE_TOO_SMALL;
     if (int e = require_sm100()) return e;
     int sms = 0;
     if (int e = current_device_sms(&sms)) return e;
@@ -732,7 +739,7 @@ int pai_gated_bwd(const void *dh, int64_t lddh, const void *x, int64_t ldx, cons
     const size_t ba = bias_fp32 ? 4 : 2;
     if (!aligned(saved, 16) || !aligned(workspace, 256) || !aligned(dw_gate, 2) || !aligned(dw_up, 2) || !aligned(db_gate, ba) || !aligned(db_up, ba))
         return PAI_ERR_MISALIGNED;
-    if (workspace_bytes < pai_dense_bwd_workspace_bytes(M, N, 1)) return PAI_ERR_WORKSPACE_TOO_SMALL;
+    if (workspace_bytes < pai_dense_bwd_workspace_bytes(M, N, K, 1)) return PAI_ERR_WORKSPACE_TOO_SMALL;
     if (int e = require_sm100()) return e;
     int sms = 0;
     if (int e = current_device_sms(&sms)) return e;
@@ -823,6 +830,7 @@ int pai_measure_sfu_peak(double *sincos_pairs_per_s, double *elapsed_ms) {
 int pai_tune_set(int key, int value) {
     if (key < 0 || key >= PAI_TUNE_COUNT) return PAI_ERR_UNSUPPORTED;
     g_tune[key] = value;
+    pai::g_dense_tune = {g_tune[PAI_TUNE_DENSE_KERNEL], g_tune[PAI_TUNE_DENSE_WIDTH], g_tune[PAI_TUNE_DENSE_SPLITS]};
     return PAI_OK;
 }
 

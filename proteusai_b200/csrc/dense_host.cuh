@@ -1,5 +1,6 @@
 // Host side of the feed-forward products: tensor maps, the choice of tile and split, the launches.
 #pragma once
+#include "dense_pair.cuh"
 #include "dense_tile.cuh"
 
 namespace pai {
@@ -36,30 +37,72 @@ struct DenseProduct {
     int bias_fp32;
     const void *residual;
     long long ld_res;
-    float *save[2];
+    void *save[2];
     int act, half;
+    float *part;               // workspace of a split reduction in the pair kernel (dense_pair_choose), or NULL: no split
 };
 
-// Tile height (rows t per CTA) and split of the reduction: the pair with the lowest estimated time.  A CTA's 64-wide reduction block costs
-// the larger of its MMAs (2 tn cycles per accumulator) and its loads (the SM takes about 48 bytes a cycle from L2); CTAs beyond one per SM
-// queue up; a split adds the exchange of partial tiles.
-static void dense_tile_choose(const DenseProduct &d, int sms, int *tn_out, int *splits_out) {
+// Test-only overrides of the choices below (0: none): kernel 1 = tile, 2 = pair; tile height / accumulator columns; split.
+struct DenseTune {
+    int kernel, width, splits;
+};
+static DenseTune g_dense_tune;
+
+// The kernel and its shape are the ones with the lowest estimated time, in cycles.
+struct DenseChoice {
+    int pair, width, splits;   // width: rows t of a tile (tile kernel), accumulator columns (pair kernel)
+    double cost;
+};
+
+// Tile kernel: a CTA's 64-wide reduction block costs the larger of its MMAs (2 tn cycles per accumulator) and its loads (the SM takes about
+// 48 bytes a cycle from L2); CTAs beyond one per SM queue up; a split adds the exchange of partial tiles.
+static DenseChoice dense_tile_choose(const DenseProduct &d, int sms) {
     const long long kb = (d.R + DT_BK - 1) / DT_BK * d.segs;
-    const int acc = d.dual ? 2 : 1;
-    double best = 1e300;
-    *tn_out = 64, *splits_out = 1;
-    for (int tn = d.b_mn ? 64 : 16; tn <= (d.dual ? 128 : 256); tn *= 2) {
-        if (tn > (d.b_mn ? 64 : 16) && tn / 2 >= d.T) break;
+    const int acc = d.dual ? 2 : 1, least = d.b_mn ? 64 : 16;
+    DenseChoice best = {0, 64, 1, 1e300};
+    for (int tn = least; tn <= (d.dual ? 128 : 256); tn *= 2) {
+        if (tn > least && tn / 2 >= d.T && g_dense_tune.width == 0) break;
+        if (g_dense_tune.kernel == 1 && g_dense_tune.width && tn != g_dense_tune.width) continue;
         const long long tiles = (d.F + DT_FT - 1) / DT_FT * ((d.T + tn - 1) / tn) * d.groups;
         for (int splits = 1; splits <= 8 && splits <= kb; splits *= 2) {
+            if (g_dense_tune.kernel == 1 && g_dense_tune.splits && splits != g_dense_tune.splits) continue;
             const double rounds = (double)((tiles * splits + sms - 1) / sms);
             const double mma = 2.0 * tn * acc, load = (128.0 * acc + tn) * 128.0 / 48.0;
             const double work = (double)((kb + splits - 1) / splits) * (mma > load ? mma : load);
             const double epi = (splits > 1 ? 1500.0 + tn * acc * 8.0 + (double)tn / splits * 20.0 * acc : tn * 12.0 * acc);
             const double t = rounds * (work + epi) + 2500.0;
-            if (t < best) best = t, *tn_out = tn, *splits_out = splits;
+            if (t < best.cost) best = {0, tn, splits, t};
         }
     }
+    return best;
+}
+
+// Pair kernel: 2 bn cycles per reduction block, one tile in flight per pair of SMs, 5000 cycles to start and to finish the last tile.  A split
+// reduction writes and reads fp32 tiles (about 2000 bytes a cycle for the whole GPU) and adds a launch.
+static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_split) {
+    const long long kb = (d.R + DT_BK - 1) / DT_BK * d.segs;
+    DenseChoice best = {1, 256, 1, 1e300};
+    for (int bn = d.dual ? 256 : 128; bn <= 256; bn *= 2) {
+        if (g_dense_tune.kernel == 2 && g_dense_tune.width && bn != g_dense_tune.width) continue;
+        const int fw = d.dual ? bn / 2 : bn;
+        const long long tiles = (d.F + fw - 1) / fw * ((d.T + 255) / 256) * d.groups;
+        for (int splits = 1; splits <= (may_split ? 16 : 1) && splits * 4 <= (kb > 4 ? kb : 4); ++splits) {
+            if (g_dense_tune.kernel == 2 && g_dense_tune.splits && may_split && splits != g_dense_tune.splits) continue;
+            const double rounds = (double)((tiles * splits + sms / 2 - 1) / (sms / 2));
+            const double block = bn == 256 ? 560.0 : 400.0, epi = bn * 14.0;
+            const double work = (double)((kb + splits - 1) / splits) * block;
+            double t = rounds * (work > epi ? work : epi) + epi + 5000.0;
+            if (splits > 1) t += 5000.0 + 2.0 * splits * d.groups * (double)d.F * d.T * 4.0 / 2000.0;
+            if (t < best.cost) best = {1, bn, splits, t};
+        }
+    }
+    return best;
+}
+
+static DenseChoice dense_choose(const DenseProduct &d, int sms, bool may_split) {
+    const DenseChoice a = dense_tile_choose(d, sms), b = dense_pair_choose(d, sms, may_split);
+    if (g_dense_tune.kernel) return g_dense_tune.kernel == 2 ? b : a;
+    return b.cost < a.cost ? b : a;
 }
 
 template <bool DUAL>
@@ -86,14 +129,17 @@ static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams
     return (int)cudaLaunchKernelEx(&cfg, dense_tile_kernel<DUAL>, m[0], m[1], m[2], m[3], p);
 }
 
-static int dense_tile_launch(const DenseProduct &d, int sms, cudaStream_t st) {
-    int tn, splits;
-    dense_tile_choose(d, sms, &tn, &splits);
+static uint32_t dense_idesc(int m, int n, const DenseProduct &d, int m_mn, int n_mn) {
+    return (umma_idesc_bf16(m, n, m_mn != 0, n_mn != 0) & ~((7u << 7) | (7u << 10))) | (d.half ? 0u : (1u << 7) | (1u << 10));
+}
+
+static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sms, cudaStream_t st) {
+    const int tn = c.width, splits = c.splits;
     DenseTileParams p = {};
     p.out0 = d.out[0], p.out1 = d.out[1];
     p.bias0 = d.bias[0], p.bias1 = d.bias[1];
     p.residual = (const unsigned short *)d.residual;
-    p.save0 = d.save[0], p.save1 = d.save[1];
+    p.save0 = (float *)d.save[0], p.save1 = (float *)d.save[1];
     p.ld_out = d.ld_out, p.ld_res = d.ld_res;
     p.F = (int)d.F, p.T = (int)d.T;
     p.f_tiles = (int)((d.F + DT_FT - 1) / DT_FT), p.t_tiles = (int)((d.T + tn - 1) / tn);
@@ -101,7 +147,7 @@ static int dense_tile_launch(const DenseProduct &d, int sms, cudaStream_t st) {
     p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
     p.a_mn = d.a_mn, p.b_mn = d.b_mn;
     p.act = d.act, p.half = d.half, p.bias_fp32 = d.bias_fp32;
-    p.idesc = (umma_idesc_bf16(128, tn, d.a_mn != 0, d.b_mn != 0) & ~((7u << 7) | (7u << 10))) | (d.half ? 0u : (1u << 7) | (1u << 10));
+    p.idesc = dense_idesc(128, tn, d, d.a_mn, d.b_mn);
     const long long ctas = (long long)p.f_tiles * p.t_tiles * d.groups * splits;
     if (ctas > 0x7fffffffll) return (int)PAI_ERR_BAD_SHAPE;
     const int stage = (d.dual ? 2 : 1) * DT_FT * 128 + tn * 128, kb_cta = (p.kb_total + splits - 1) / splits;
@@ -123,22 +169,120 @@ static int dense_tile_launch(const DenseProduct &d, int sms, cudaStream_t st) {
     return d.dual ? dense_tile_launch_as<true>(m, p, ctas, smem, st) : dense_tile_launch_as<false>(m, p, ctas, smem, st);
 }
 
+// map of an operand as MMA rows (`rows` of them, `box` per load): reduction-contiguous or not
+static int make_operand_map(CUtensorMap *m, const DenseOperand &o, int mn, long long rows, long long R, int box, int half) {
+    return mn ? make_map_16(m, o.p, rows, R, o.ld, 64, half) : make_map_16(m, o.p, R, rows, o.ld, box, half);
+}
+
+template <int MODE>
+static int dense_pair_launch_as(const CUtensorMap (&m)[6], const DensePairParams &p, int ctas, cudaStream_t st) {
+    static bool attr_done[64];
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev < 0 || dev >= 64 || !attr_done[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DensePairSmem));
+        if (e != cudaSuccess) return (int)e;
+        if (dev >= 0 && dev < 64) attr_done[dev] = true;
+    }
+    dense_pair_kernel<MODE><<<ctas, DP_THREADS, sizeof(DensePairSmem), st>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
+    return (int)cudaPeekAtLastError();
+}
+
+// (in the roles of DenseProduct the pair kernel's rows are t, its columns f: its A is `b`, its B is `a`)
+static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sms, cudaStream_t st) {
+    if (d.groups > 1 && c.splits == 1) {  // two whole products: one output map each
+        for (int g = 0; g < d.groups; ++g) {
+            DenseProduct e = d;
+            e.groups = 1;
+            e.b[0] = d.b[g], e.b[1] = {nullptr, 0};
+            e.out[0] = d.out[g], e.out[1] = nullptr;
+            if (int r = dense_pair_launch(e, c, sms, st)) return r;
+        }
+        return 0;
+    }
+    DensePairParams p = {};
+    const int fw = d.dual ? c.width / 2 : c.width;
+    p.out0 = (unsigned short *)d.out[0];
+    p.residual = (const unsigned short *)d.residual;
+    p.bias0 = d.bias[0], p.bias1 = d.bias[1], p.bias_fp32 = d.bias_fp32;
+    p.save0 = (uint8_t *)d.save[0], p.save1 = (uint8_t *)d.save[1];
+    p.save_f32 = d.half;
+    p.save_scale_off = (long long)saved_blocks(d.T, (int)d.F) * 2048;
+    p.part = d.part;
+    p.ld_out = d.ld_out, p.ld_res = d.ld_res;
+    p.T = (int)d.T, p.F = (int)d.F, p.bn = c.width;
+    p.t_tiles = (int)((d.T + 255) / 256), p.f_tiles = (int)((d.F + fw - 1) / fw), p.groups = d.groups, p.splits = c.splits;
+    p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
+    p.a_mn = d.b_mn, p.b_mn = d.a_mn, p.act = d.act, p.half = d.half;
+    p.idesc = dense_idesc(256, c.width, d, d.b_mn, d.a_mn);
+    const long long items = (long long)p.t_tiles * p.f_tiles * p.groups * p.splits;
+    if (items > 0x3fffffffll) return (int)PAI_ERR_BAD_SHAPE;
+    CUtensorMap m[6];
+    for (int i = 0; i < 2; ++i) {
+        if (i == 1 && !d.b[1].p) m[1] = m[0];
+        else if (int e = make_operand_map(&m[i], d.b[i], d.b_mn, d.T, d.R, 128, d.half)) return e;
+        if (i == 1 && !d.a[1].p) m[3] = m[2];
+        else if (int e = make_operand_map(&m[2 + i], d.a[i], d.a_mn, d.F, d.R, c.width / 2, d.half)) return e;
+    }
+    m[4] = m[5] = m[0];
+    const bool partial = c.splits > 1;
+    p.tma_out = !partial && ((uintptr_t)d.out[0] & 15) == 0 && (d.T == 1 || (d.ld_out & 7) == 0);
+    if (p.tma_out)
+        if (int e = make_map_16(&m[4], d.out[0], d.F, d.T, d.ld_out, 32, d.half)) return e;
+    p.tma_res = d.residual && ((uintptr_t)d.residual & 15) == 0 && (d.T == 1 || ((d.ld_res & 7) == 0 && d.ld_res >= d.F));
+    if (p.tma_res)
+        if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half)) return e;
+    const int ctas = 2 * (int)(items < sms / 2 ? items : sms / 2);
+    if (partial) {
+        if (int e = dense_pair_launch_as<DP_PARTIAL>(m, p, ctas, st)) return e;
+        const size_t blocks = saved_blocks(d.T, (int)d.F);
+        dense_reduce_kernel<<<dim3((unsigned)((blocks + 7) / 8), d.groups), 256, 0, st>>>(d.part, (unsigned short *)d.out[0], (unsigned short *)d.out[1],
+                                                                                        p.T, p.F, d.ld_out, d.groups, c.splits, d.half);
+        return (int)cudaPeekAtLastError();
+    }
+    return d.dual ? dense_pair_launch_as<DP_GATED>(m, p, ctas, st) : dense_pair_launch_as<DP_LINEAR>(m, p, ctas, st);
+}
+
+static int dense_launch(const DenseProduct &d, int sms, cudaStream_t st) {
+    const DenseChoice c = dense_choose(d, sms, d.part != nullptr);
+    return c.pair ? dense_pair_launch(d, c, sms, st) : dense_tile_launch(d, c, sms, st);
+}
+
+// The products as problems (sizes only): what the saved buffer and the workspace are sized for, and what runs.
+static DenseProduct dense_forward_product(long long M, int N, int K, int gated) {
+    DenseProduct d = {};
+    d.dual = gated, d.segs = 1, d.groups = 1;
+    d.F = N, d.T = M, d.R = K;
+    return d;
+}
+static DenseProduct dense_weight_product(long long M, int N, int K, int groups) {
+    DenseProduct d = {};
+    d.a_mn = 1, d.b_mn = 1, d.segs = 1, d.groups = groups;
+    d.F = K, d.T = N, d.R = M;
+    return d;
+}
+// the form of the saved pre-activations: fp16 with exponents where the pair kernel runs on bf16, fp32 otherwise
+static bool dense_saves_f32(long long M, int N, int K, int gated, int half, int sms) {
+    return half || !dense_choose(dense_forward_product(M, N, K, gated), sms, false).pair;
+}
+static size_t dense_saved_matrix(long long M, int N, int K, int gated, int half, int sms) {
+    return dense_saves_f32(M, N, K, gated, half, sms) ? saved_bytes_f32(M, N) : saved_bytes_f16(M, N);
+}
+
 // ---- the two operators ----------------------------------------------------------------------------------------------
 static int dense_forward(const DenseOperand &x, const DenseOperand (&w)[2], const void *const (&bias)[2], int bias_fp32, const DenseOperand &residual,
                          void *y, long long ldy, void *saved, long long M, int N, int K, int act, int half, int sms, cudaStream_t st) {
-    DenseProduct d = {};
     const bool gated = w[1].p != nullptr;
+    DenseProduct d = dense_forward_product(M, N, K, gated);
     d.a[0] = w[0], d.a[1] = w[1];
     d.b[0] = x;
-    d.dual = gated, d.segs = 1, d.groups = 1;
-    d.F = N, d.T = M, d.R = K;
     d.out[0] = y, d.ld_out = ldy;
     d.bias[0] = bias[0], d.bias[1] = bias[1], d.bias_fp32 = bias_fp32;
     d.residual = residual.p, d.ld_res = residual.ld;
-    d.save[0] = (float *)saved;
-    d.save[1] = saved && gated ? (float *)((char *)saved + saved_bytes_f32(M, N)) : nullptr;
+    d.save[0] = saved;
+    d.save[1] = saved && gated ? (char *)saved + dense_saved_matrix(M, N, K, gated, half, sms) : nullptr;
     d.act = act, d.half = half;
-    return dense_tile_launch(d, sms, st);
+    return dense_launch(d, sms, st);
 }
 
 // Strips of the elementwise pass: about four CTAs of 256 threads per SM, at least 64 rows each.
@@ -153,10 +297,20 @@ inline long long dense_strips(long long M, int N) {
     return (M + s - 1) / s;
 }
 inline size_t align256(size_t b) { return (b + 255) / 256 * 256; }
-// workspace: the 16-bit gradient(s) of the pre-activations, then the strips' column sums
+// workspace: the 16-bit gradient(s) of the pre-activations, the strips' column sums, the fp32 tiles of a split weight gradient
 inline size_t dense_d_bytes(long long M, int N) { return align256((size_t)M * dense_ld16(N) * 2); }
-inline size_t dense_bwd_workspace(long long M, int N, int mats) {
-    return mats * (dense_d_bytes(M, N) + align256((size_t)dense_strips(M, N) * N * 4));
+inline size_t dense_part_bytes(long long M, int N) { return align256((size_t)dense_strips(M, N) * N * 4); }
+static size_t dense_split_bytes(long long M, int N, int K, int mats, int sms) {
+    size_t most = 0;
+    for (int g = 1; g <= mats; ++g) {  // (one of the two weight gradients alone may split further)
+        const DenseChoice c = dense_choose(dense_weight_product(M, N, K, g), sms, true);
+        const size_t b = c.pair && c.splits > 1 ? (size_t)c.splits * g * saved_bytes_f32(N, K) : 0;
+        most = b > most ? b : most;
+    }
+    return most;
+}
+static size_t dense_bwd_workspace(long long M, int N, int K, int mats, int sms) {
+    return mats * (dense_d_bytes(M, N) + dense_part_bytes(M, N)) + dense_split_bytes(M, N, K, mats, sms);
 }
 
 static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const DenseOperand (&w)[2], const void *saved, void *dx, long long lddx,
@@ -174,8 +328,10 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
     p.vec_dy = ((uintptr_t)dy.p & 15) == 0 && (dy.ld & 7) == 0;
     p.M = M, p.N = N, p.act = act, p.half = half, p.strip = dense_strip_rows(M, N);
     if (elementwise) {
-        p.save0 = (const float *)saved;
-        p.save1 = gated ? (const float *)((const char *)saved + saved_bytes_f32(M, N)) : nullptr;
+        p.save0 = (const uint8_t *)saved;
+        p.save1 = gated ? (const uint8_t *)saved + dense_saved_matrix(M, N, K, gated, half, sms) : nullptr;
+        p.save_f32 = dense_saves_f32(M, N, K, gated, half, sms);
+        p.save_exps = saved_blocks(M, N) * 2048;
         if (products) {
             p.ld_d = dense_ld16(N);
             p.d0 = (unsigned short *)ws;
@@ -185,7 +341,7 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
     }
     if (db[0] || db[1]) {
         p.part0 = (float *)(ws + mats * dense_d_bytes(M, N));
-        p.part1 = gated ? p.part0 + align256((size_t)strips * N * 4) / 4 : nullptr;
+        p.part1 = gated ? p.part0 + dense_part_bytes(M, N) / 4 : nullptr;
     }
     if ((elementwise && products) || p.part0) {
         const dim3 grid((N + 255) / 256, (unsigned)strips);
@@ -208,17 +364,16 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
         d.segs = mats, d.groups = 1;
         d.F = K, d.T = M, d.R = N;
         d.out[0] = dx, d.ld_out = lddx, d.half = half;
-        if (int e = dense_tile_launch(d, sms, st)) return e;
+        if (int e = dense_launch(d, sms, st)) return e;
     }
     if (dw[0] || dw[1]) {
-        DenseProduct d = {};
-        d.a[0] = x, d.a_mn = 1, d.b_mn = 1;
-        d.segs = 1, d.groups = dw[0] && dw[1] ? 2 : 1;
+        DenseProduct d = dense_weight_product(M, N, K, dw[0] && dw[1] ? 2 : 1);
+        d.a[0] = x;
         d.b[0] = dw[0] ? dz[0] : dz[1], d.out[0] = dw[0] ? dw[0] : dw[1];
         if (d.groups == 2) d.b[1] = dz[1], d.out[1] = dw[1];
-        d.F = K, d.T = N, d.R = M;
         d.ld_out = K, d.half = half;
-        if (int e = dense_tile_launch(d, sms, st)) return e;
+        d.part = (float *)(ws + mats * (dense_d_bytes(M, N) + dense_part_bytes(M, N)));
+        if (int e = dense_launch(d, sms, st)) return e;
     }
     return 0;
 }

@@ -26,45 +26,47 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // log2 Phi(-a), a >= 0, as a polynomial of degree 7: Chebyshev fit of log2 of the normal distribution function on [0, 6], so that
 // 2^p has a RELATIVE error below 4e-6 there (half a bf16 step is 2^-9 .. 2^-8, half an fp16 step 2^-12 .. 2^-11).  Beyond 6 it keeps
 // falling (its leading coefficient is negative), where x Phi(x) is below 1e-8 in magnitude: the absolute error of x Phi(x) stays
-// below 6e-7 on the whole negative axis.  One SFU operation, against two for the rational form of erfc.
+// below 6e-7 on the whole negative axis.  One SFU operation, against two for the rational form of erfc.  a is cut off at 30, where
+// Phi(-a) is 0 in fp32, so that infinities do not meet that 0.
 #define PAI_PHI_COEFFS                                                                                                    \
     {-9.999943403e-01f, -1.151269147e+00f, -4.584097768e-01f, -5.402068712e-02f, 8.539461332e-03f, -9.388679333e-04f, \
      6.268140101e-05f,  -1.889626234e-06f}
 
-__device__ __forceinline__ float normal_cdf(float x) {
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+// Phi(-min(|x|, 30))
+__device__ __forceinline__ float normal_tail(float a) {
     constexpr float c[8] = PAI_PHI_COEFFS;
-    const float a = fabsf(x);
     float p = c[7];
 #pragma unroll
     for (int i = 6; i >= 0; --i) p = fmaf(p, a, c[i]);
-    const float e = ex2_approx(p);
-    return x < 0.f ? e : 1.f - e;
+    return ex2_approx(p);
 }
-// the same for a pair, the polynomial in packed arithmetic
-__device__ __forceinline__ void normal_cdf2(float x0, float x1, float &phi0, float &phi1) {
+// x Phi(x) = max(x, 0) - |x| Phi(-|x|) for a pair, the polynomial in packed arithmetic
+__device__ __forceinline__ void gelu2(float &x0, float &x1) {
     constexpr float c[8] = PAI_PHI_COEFFS;
-    const f2_t a = f2_pack(fabsf(x0), fabsf(x1));
+    const f2_t a = f2_pack(fminf(fabsf(x0), 30.f), fminf(fabsf(x1), 30.f));
     f2_t p = f2_pack(c[7], c[7]);
 #pragma unroll
     for (int i = 6; i >= 0; --i) p = f2_fma(p, a, f2_pack(c[i], c[i]));
     float p0, p1;
     f2_unpack(p, p0, p1);
-    const float e0 = ex2_approx(p0), e1 = ex2_approx(p1);
-    phi0 = x0 < 0.f ? e0 : 1.f - e0;
-    phi1 = x1 < 0.f ? e1 : 1.f - e1;
+    const f2_t e = f2_pack(-ex2_approx(p0), -ex2_approx(p1));
+    f2_unpack(f2_fma(a, e, f2_pack(max_nan(x0, 0.f), max_nan(x1, 0.f))), x0, x1);
 }
 __device__ __forceinline__ float sigmoid_f(float x) { return rcp_approx(1.f + ex2_approx(-1.4426950408889634f * x)); }
 
 template <int ACT>
 __device__ __forceinline__ void act_pair(float &a, float &b) {
     if (ACT == ACT_GELU) {
-        float pa, pb;
-        normal_cdf2(a, b, pa, pb);
-        a *= pa, b *= pb;
+        gelu2(a, b);
     } else if (ACT == ACT_SILU) {
         a *= sigmoid_f(a), b *= sigmoid_f(b);
     } else if (ACT == ACT_RELU) {
-        a = a < 0.f ? 0.f : a, b = b < 0.f ? 0.f : b;  // (a NaN stays one)
+        a = max_nan(a, 0.f), b = max_nan(b, 0.f);
     } else if (ACT == ACT_SIGMOID) {
         a = sigmoid_f(a), b = sigmoid_f(b);
     }
@@ -74,8 +76,8 @@ __device__ __forceinline__ void act_pair(float &a, float &b) {
 __device__ __forceinline__ void act_and_slope(int act, float z, float &a, float &d) {
     switch (act) {
         case ACT_GELU: {
-            const float phi = normal_cdf(z);
-            a = z * phi;
+            const float t = fminf(fabsf(z), 30.f), e = normal_tail(t), phi = z < 0.f ? e : 1.f - e;
+            a = fmaf(-t, e, max_nan(z, 0.f));
             d = fmaf(z * 0.3989422804014327f, ex2_approx(-0.7213475204444817f * z * z), phi);
             break;
         }
@@ -86,7 +88,7 @@ __device__ __forceinline__ void act_and_slope(int act, float z, float &a, float 
             break;
         }
         case ACT_RELU:
-            a = z < 0.f ? 0.f : z;
+            a = max_nan(z, 0.f);
             d = z > 0.f ? 1.f : 0.f;
             break;
         case ACT_SIGMOID:
@@ -122,13 +124,37 @@ __device__ __forceinline__ void unpack_bits16(uint32_t w, int half, float &lo, f
 }
 
 // ---- saved pre-activations ----------------------------------------------------------------------------------------
-// What the backward pass needs besides its inputs is z (linear, with an activation) or g and u (gated).  Rounding them to the
-// tensors' own 16-bit type would add an error as large as the outputs' rounding; they are kept in fp32, in blocks of 32 rows x 32
-// columns laid out [piece of 4 columns][row][4]: both a thread per row and a thread per column write whole sectors.
+// What the backward pass needs besides its inputs is z (linear, with an activation) or g and u (gated).  Rounding them to the tensors'
+// own 16-bit type would add an error as large as the outputs' rounding, so they are kept in more bits, in blocks of 32 rows x 32 columns:
+//   fp32   [piece of 4 columns][row][4]: a thread per row and a thread per column both write whole sectors
+//   fp16   (bf16 tensors, dense_pair.cuh) [piece of 8 columns][row][8] with one power of two per row and 32 columns, chosen so that the largest
+//          magnitude of the run lies in [2^14, 2^15): 2^-12 relative accuracy for everything within 2^-28 of it, in 16 bits.  The exponents
+//          (int8, [block][row]) follow the values.
 __host__ __device__ inline size_t saved_blocks(long long rows, int cols) { return (size_t)((rows + 31) / 32) * (size_t)((cols + 31) / 32); }
 __host__ __device__ inline size_t saved_bytes_f32(long long rows, int cols) { return saved_blocks(rows, cols) * 4096; }
+__host__ __device__ inline size_t saved_bytes_f16(long long rows, int cols) { return saved_blocks(rows, cols) * (2048 + 32); }
+__device__ __forceinline__ size_t saved_block(long long row, int col, int col_blocks) { return (size_t)(row >> 5) * col_blocks + (col >> 5); }
 __device__ __forceinline__ size_t saved_index_f32(long long row, int col, int col_blocks) {
-    return (((size_t)(row >> 5) * col_blocks + (col >> 5)) * 8 + ((col & 31) >> 2)) * 128 + (size_t)(row & 31) * 4 + (col & 3);
+    return (saved_block(row, col, col_blocks) * 8 + ((col & 31) >> 2)) * 128 + (size_t)(row & 31) * 4 + (col & 3);
+}
+// eight columns (col a multiple of 8) of a row
+__device__ __forceinline__ void saved_load8(const uint8_t *save, int f32, size_t exps, long long row, int col, int col_blocks, float (&z)[8]) {
+    if (f32) {
+        const float *src = reinterpret_cast<const float *>(save) + saved_index_f32(row, col, col_blocks);
+        const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 128);
+        z[0] = a.x, z[1] = a.y, z[2] = a.z, z[3] = a.w, z[4] = b.x, z[5] = b.y, z[6] = b.z, z[7] = b.w;
+    } else {
+        const size_t block = saved_block(row, col, col_blocks);
+        const uint4 v = *reinterpret_cast<const uint4 *>(save + block * 2048 + ((col & 31) >> 3) * 512 + (row & 31) * 16);
+        const int e = reinterpret_cast<const signed char *>(save)[exps + block * 32 + (row & 31)];
+        const float s = __uint_as_float((uint32_t)(127 + e) << 23);
+        unpack_bits16(v.x, 1, z[0], z[1]);
+        unpack_bits16(v.y, 1, z[2], z[3]);
+        unpack_bits16(v.z, 1, z[4], z[5]);
+        unpack_bits16(v.w, 1, z[6], z[7]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] *= s;
+    }
 }
 
 // ---- elementwise half of the backward pass ------------------------------------------------------------------------
@@ -139,7 +165,9 @@ __device__ __forceinline__ size_t saved_index_f32(long long row, int col, int co
 struct DenseBwdElemParams {
     const unsigned short *dy;
     long long ld_dy;
-    const float *save0, *save1;     // z, or g and u
+    const uint8_t *save0, *save1;   // z, or g and u
+    size_t save_exps;               // fp16 form: offset of the exponents
+    int save_f32;
     unsigned short *d0, *d1;        // dz, or dg and du; NULL: not wanted (d0: sums of dy alone)
     long long ld_d;
     float *part0, *part1;           // [strips, N] column sums, or NULL
@@ -174,12 +202,11 @@ __global__ void __launch_bounds__(256) dense_bwd_elem_kernel(const __grid_consta
             }
             float o0[8], o1[8];
             if (p.save0) {
-                const size_t at = saved_index_f32(r, c0, col_blocks);
-                const float4 za = *reinterpret_cast<const float4 *>(p.save0 + at), zb = *reinterpret_cast<const float4 *>(p.save0 + at + 128);
-                const float z[8] = {za.x, za.y, za.z, za.w, zb.x, zb.y, zb.z, zb.w};
+                float z[8];
+                saved_load8(p.save0, p.save_f32, p.save_exps, r, c0, col_blocks, z);
                 if (DUAL) {
-                    const float4 ua = *reinterpret_cast<const float4 *>(p.save1 + at), ub = *reinterpret_cast<const float4 *>(p.save1 + at + 128);
-                    const float u[8] = {ua.x, ua.y, ua.z, ua.w, ub.x, ub.y, ub.z, ub.w};
+                    float u[8];
+                    saved_load8(p.save1, p.save_f32, p.save_exps, r, c0, col_blocks, u);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         float a, d;

@@ -118,7 +118,7 @@ def _forward(x, ws, bs, r, act, save):
         return y, saved
     lib = _lib.lib()
     if save and (gated or act):
-        saved = torch.empty(lib.pai_dense_saved_bytes(m, n, gated), dtype=torch.uint8, device=x.device)
+        saved = torch.empty(lib.pai_dense_saved_bytes(m, n, k, gated, _DTYPES[x.dtype]), dtype=torch.uint8, device=x.device)
     fp32 = any(b is not None and b.dtype == torch.float32 for b in bs)
     with _on(x) as stream:
         if gated:
@@ -148,7 +148,7 @@ def _backward(dy, x, ws, bs, saved, act, need_x, need_w, need_b):
         dy = _operand(dy)
     lib = _lib.lib()
     fp32 = any(b is not None and b.dtype == torch.float32 for b in bs)
-    size = lib.pai_dense_bwd_workspace_bytes(m, n, gated)
+    size = lib.pai_dense_bwd_workspace_bytes(m, n, k, gated)
     ws_buf = torch.empty(size, dtype=torch.uint8, device=x.device)
     with _on(x) as stream:
         if gated:

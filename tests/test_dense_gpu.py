@@ -128,3 +128,26 @@ def test_gated_linear_and_gradients(m, k, n, dtype):
     for i, act in enumerate(ACTS):
         x, ws, bs, _, dy = _inputs(m, k, n, dtype, 2, (m + i) % 3 != 0, False, seed=20 + i)
         _check(_run(x, ws, bs, None, dy, act), _expected(x, ws, bs, None, dy, act), dtype, f"{act}")
+
+
+@pytest.fixture
+def tuned():
+    from proteusai_b200 import _lib
+    yield _lib.tune
+    _lib.tune_reset()
+
+
+# Every kernel and shape at sizes that cross its borders, whichever the library would have chosen: a tile, less than one, several.
+VARIANTS = [("tile", w, s) for w in (16, 64, 128, 256) for s in (1, 8)] + [("pair", 128, 1), ("pair", 256, 1), ("pair", 256, 3)]
+
+
+@pytest.mark.parametrize("kernel,width,splits", VARIANTS)
+@pytest.mark.parametrize("m,k,n", [(5, 40, 24), (256, 64, 256), (333, 321, 263), (700, 520, 640)])
+def test_kernel_variants(tuned, kernel, width, splits, m, k, n):
+    tuned(dense_kernel=1 if kernel == "tile" else 2, dense_width=width, dense_splits=splits)
+    for dtype in DTYPES:
+        for act, residual in ((None, True), ("gelu", False), ("silu", True)):
+            x, ws, bs, r, dy = _inputs(m, k, n, dtype, 1, True, residual, seed=3)
+            _check(_run(x, ws, bs, r, dy, act), _expected(x, ws, bs, r, dy, act), dtype, f"{act}")
+        x, ws, bs, _, dy = _inputs(m, k, n, dtype, 2, True, False, seed=4)
+        _check(_run(x, ws, bs, None, dy, "gelu"), _expected(x, ws, bs, None, dy, "gelu"), dtype, "gated")
