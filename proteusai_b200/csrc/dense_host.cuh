@@ -7,16 +7,18 @@ namespace pai {
 
 inline long long dense_ld16(long long cols) { return (cols + 7) / 8 * 8; }  // row pitch of a 16-bit workspace matrix
 
-// Map of a [rows, inner] matrix of 16-bit elements with row pitch `ld` elements, boxes of 64 x box_rows; outside reads as 0.
-static int make_map_16(CUtensorMap *map, const void *base, long long inner, long long rows, long long ld, int box_rows, int half) {
+// Map of a [rows, inner] matrix of 16-bit elements with row pitch `ld` elements, boxes of box_rows rows x 64 columns (128-byte swizzle) or 32 (64-byte
+// swizzle); outside reads as 0.
+static int make_map_16(CUtensorMap *map, const void *base, long long inner, long long rows, long long ld, int box_rows, int half, int box_cols = 64) {
     EncodeTiledFn enc = get_encode_tiled();
     if (!enc) return (int)PAI_ERR_UNSUPPORTED;
     cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)(rows > 1 ? ld : dense_ld16(inner)) * 2};
-    cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
     CUresult r = enc(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box,
-                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : (int)PAI_ERR_UNSUPPORTED;
 }
@@ -207,7 +209,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     p.bias0 = d.bias[0], p.bias1 = d.bias[1], p.bias_fp32 = d.bias_fp32;
     p.save0 = (uint8_t *)d.save[0], p.save1 = (uint8_t *)d.save[1];
     p.save_f32 = d.half;
-    p.save_scale_off = (long long)saved_blocks(d.T, (int)d.F) * 2048;
+    p.save_exps = (long long)saved_blocks(d.T, (int)d.F) * 2048;
     p.part = d.part;
     p.ld_out = d.ld_out, p.ld_res = d.ld_res;
     p.T = (int)d.T, p.F = (int)d.F, p.bn = c.width;
@@ -228,10 +230,10 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     const bool partial = c.splits > 1;
     p.tma_out = !partial && ((uintptr_t)d.out[0] & 15) == 0 && (d.T == 1 || (d.ld_out & 7) == 0);
     if (p.tma_out)
-        if (int e = make_map_16(&m[4], d.out[0], d.F, d.T, d.ld_out, 32, d.half)) return e;
+        if (int e = make_map_16(&m[4], d.out[0], d.F, d.T, d.ld_out, 32, d.half, fw / 4)) return e;
     p.tma_res = d.residual && ((uintptr_t)d.residual & 15) == 0 && (d.T == 1 || ((d.ld_res & 7) == 0 && d.ld_res >= d.F));
     if (p.tma_res)
-        if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half)) return e;
+        if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half, fw / 4)) return e;
     const int ctas = 2 * (int)(items < sms / 2 ? items : sms / 2);
     if (partial) {
         if (int e = dense_pair_launch_as<DP_PARTIAL>(m, p, ctas, st)) return e;

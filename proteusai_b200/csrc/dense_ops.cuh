@@ -127,12 +127,12 @@ __device__ __forceinline__ void unpack_bits16(uint32_t w, int half, float &lo, f
 // What the backward pass needs besides its inputs is z (linear, with an activation) or g and u (gated).  Rounding them to the tensors'
 // own 16-bit type would add an error as large as the outputs' rounding, so they are kept in more bits, in blocks of 32 rows x 32 columns:
 //   fp32   [piece of 4 columns][row][4]: a thread per row and a thread per column both write whole sectors
-//   fp16   (bf16 tensors, dense_pair.cuh) [piece of 8 columns][row][8] with one power of two per row and 32 columns, chosen so that the largest
+//   fp16   (bf16 tensors, dense_pair.cuh) [piece of 8 columns][row][8] with one power of two per row and 16 columns, chosen so that the largest
 //          magnitude of the run lies in [2^14, 2^15): 2^-12 relative accuracy for everything within 2^-28 of it, in 16 bits.  The exponents
-//          (int8, [block][row]) follow the values.
+//          (int8, [block][half][row]) follow the values.
 __host__ __device__ inline size_t saved_blocks(long long rows, int cols) { return (size_t)((rows + 31) / 32) * (size_t)((cols + 31) / 32); }
 __host__ __device__ inline size_t saved_bytes_f32(long long rows, int cols) { return saved_blocks(rows, cols) * 4096; }
-__host__ __device__ inline size_t saved_bytes_f16(long long rows, int cols) { return saved_blocks(rows, cols) * (2048 + 32); }
+__host__ __device__ inline size_t saved_bytes_f16(long long rows, int cols) { return saved_blocks(rows, cols) * (2048 + 64); }
 __device__ __forceinline__ size_t saved_block(long long row, int col, int col_blocks) { return (size_t)(row >> 5) * col_blocks + (col >> 5); }
 __device__ __forceinline__ size_t saved_index_f32(long long row, int col, int col_blocks) {
     return (saved_block(row, col, col_blocks) * 8 + ((col & 31) >> 2)) * 128 + (size_t)(row & 31) * 4 + (col & 3);
@@ -146,7 +146,7 @@ __device__ __forceinline__ void saved_load8(const uint8_t *save, int f32, size_t
     } else {
         const size_t block = saved_block(row, col, col_blocks);
         const uint4 v = *reinterpret_cast<const uint4 *>(save + block * 2048 + ((col & 31) >> 3) * 512 + (row & 31) * 16);
-        const int e = reinterpret_cast<const signed char *>(save)[exps + block * 32 + (row & 31)];
+        const int e = reinterpret_cast<const signed char *>(save)[exps + block * 64 + ((col & 31) >> 4) * 32 + (row & 31)];
         const float s = __uint_as_float((uint32_t)(127 + e) << 23);
         unpack_bits16(v.x, 1, z[0], z[1]);
         unpack_bits16(v.y, 1, z[2], z[3]);

@@ -13,23 +13,25 @@
 //     dW       t = output feature,  f = input feature,  r = token:          A = dz (MN-major), B = x (MN-major); the long reduction split
 //              over pairs that leave fp32 tiles in the workspace, added in order by dense_reduce_kernel
 //
-// Warps: 0 TMA loads, 1 MMAs (first CTA of the pair), 2 tensor memory, 4..11 epilogue (two per quarter of the lanes, half the columns each).
+// Warps: 0 TMA loads, 1 MMAs (first CTA of the pair), 2 tensor memory, 4..19 epilogue (four per quarter of the lanes, a quarter of the
+// columns each: the epilogue is a chain of latencies, and with eight warps and a barrier per tile it took three times as long as the products
+// of a short reduction).
 #pragma once
 #include "dense_tile.cuh"
 
 namespace pai {
 
-constexpr int DP_THREADS = 384;
+constexpr int DP_THREADS = 640;
 constexpr int DP_STAGES = 5;
 constexpr int DP_STAGE_BYTES = 32768;  // A 128 x 128 bytes, B up to 128 x 128 bytes
-constexpr int DP_EPI_WARPS = 8;
+constexpr int DP_EPI_WARPS = 16;
 
 struct DensePairSmem {
     uint8_t stage[DP_STAGES][DP_STAGE_BYTES];
-    uint8_t panel[DP_EPI_WARPS][2][4096];  // per epilogue warp: 32 rows x 128 bytes, 128-byte swizzle; output (and residual) staging
+    uint8_t panel[DP_EPI_WARPS][4096];  // per epilogue warp: 32 rows x 64 (128-byte swizzle) or 32 columns (64-byte swizzle); output and residual
     float bias[2][256];
     uint64_t full[DP_STAGES], free[DP_STAGES], acc_full[2], acc_free[2];
-    uint64_t res_full[DP_EPI_WARPS][2];
+    uint64_t res_full[DP_EPI_WARPS];
     uint32_t tmem;
     int abort_flag;
 };
@@ -42,7 +44,7 @@ struct DensePairParams {
     const void *bias0, *bias1;
     uint8_t *save0, *save1;          // saved pre-activations of g / z and u, or NULL
     float *part;                     // DP_PARTIAL: fp32 tiles, [split][group] matrices in the layout of saved_index_f32
-    long long ld_out, ld_res, save_scale_off;
+    long long ld_out, ld_res, save_exps;
     int T, F, bn;                    // bn: accumulator columns of a tile (gated: bn / 2 of each)
     int t_tiles, f_tiles, groups, splits;
     int kb_seg, kb_total;
@@ -61,6 +63,12 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
     uint32_t r;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
+}
+// one thread of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 // load into this CTA's shared memory, completion on a barrier of either CTA of the pair (`bar`: shared::cluster address)
 __device__ __forceinline__ void tma_load_2d_pair(void *dst_smem, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
@@ -96,213 +104,216 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t *bar) {
                  : "memory");
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 // ---- epilogue -------------------------------------------------------------------------------------------------------
-// v[i] (32 columns of this thread's row) to the block; NaN and infinities keep their kind
-__device__ __forceinline__ void save_run_f16(uint8_t *values, uint8_t *exps, size_t block, int row, const float (&v)[32]) {
+// v[i]: 16 columns (from `col`, a multiple of 16) of row `row` of a block of saved pre-activations; NaN and infinities keep their kind
+__device__ __forceinline__ void save_run_f16(uint8_t *values, uint8_t *exps, size_t block, int col, int row, const float (&v)[16]) {
     float m = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) m = fmaxf(m, fabsf(v[i]));
+    for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
     int e = (int)(__float_as_uint(m) >> 23) - 127 - 14;  // 2^e 2^14 <= m < 2^e 2^15
     if (m == 0.f || m > 3.4e38f) e = 0;
     e = e < -112 ? -112 : e;  // (2^-e stays finite; what is smaller than 2^-98 loses bits)
     const float s = __uint_as_float((uint32_t)(127 - e) << 23);
-    uint4 *dst = reinterpret_cast<uint4 *>(values + block * 2048);
+    uint4 *dst = reinterpret_cast<uint4 *>(values + block * 2048) + ((col & 31) >> 3) * 32 + row;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < 2; ++q) {
         uint32_t w[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = pack_bits16(v[q * 8 + 2 * i] * s, v[q * 8 + 2 * i + 1] * s, 1);
-        dst[q * 32 + row] = make_uint4(w[0], w[1], w[2], w[3]);
+        dst[q * 32] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    exps[block * 32 + row] = (uint8_t)(signed char)e;
+    exps[block * 64 + ((col & 31) >> 4) * 32 + row] = (uint8_t)(signed char)e;
 }
-__device__ __forceinline__ void save_run_f32(float *values, size_t block, int row, const float (&v)[32]) {
-    float4 *dst = reinterpret_cast<float4 *>(values + block * 1024);
+__device__ __forceinline__ void save_run_f32(float *values, size_t block, int col, int row, const float (&v)[16]) {
+    float4 *dst = reinterpret_cast<float4 *>(values + block * 1024) + ((col & 31) >> 2) * 32 + row;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) dst[q * 32 + row] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+    for (int q = 0; q < 4; ++q) dst[q * 32] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
-
-__device__ __forceinline__ void load_run(uint32_t taddr, float (&v)[32]) {
-    uint32_t u[32];
-    tmem_ld32(taddr, u);
-    tmem_wait_ld();
+__device__ __forceinline__ void add_bias_run(float (&v)[16], const float *bias) {
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(u[i]);
-}
-__device__ __forceinline__ void add_bias_run(float (&v)[32], const float *bias) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 4; ++i) {
         const float4 b = reinterpret_cast<const float4 *>(bias)[i];
-        v[4 * i] += b.x, v[4 * i + 1] += b.y, v[4 * i + 2] += b.z, v[4 * i + 3] += b.w;
+        f2_unpack(f2_add(f2_pack(v[4 * i], v[4 * i + 1]), f2_pack(b.x, b.y)), v[4 * i], v[4 * i + 1]);
+        f2_unpack(f2_add(f2_pack(v[4 * i + 2], v[4 * i + 3]), f2_pack(b.z, b.w)), v[4 * i + 2], v[4 * i + 3]);
     }
 }
 
-// One 64-column panel of the tile for one warp: accumulators at `acc` (and `acc2`), output columns c0 .. c0 + 63 of rows row0 .. row0 + 31.
+// The tiles of a pair in turn: item = pair + n pairs in the order (f fastest, t, group, split).  Stepping adds the digits of `pairs` with carries: a
+// division per tile would cost the one thread that issues the products several hundred cycles between tiles.
+struct DensePairTiles {
+    int f, t, gs;             // digits of the current item (gs = split * groups + group)
+    int step_f, step_t, step_gs;
+    __device__ __forceinline__ DensePairTiles(const DensePairParams &p, int item, int pairs) {
+        f = item % p.f_tiles, t = item / p.f_tiles, gs = t / p.t_tiles, t %= p.t_tiles;
+        step_f = pairs % p.f_tiles, step_t = pairs / p.f_tiles, step_gs = step_t / p.t_tiles, step_t %= p.t_tiles;
+    }
+    __device__ __forceinline__ bool valid(const DensePairParams &p) const { return gs < p.groups * p.splits; }
+    __device__ __forceinline__ void next(const DensePairParams &p) {
+        f += step_f, t += step_t, gs += step_gs;
+        if (f >= p.f_tiles) f -= p.f_tiles, ++t;
+        if (t >= p.t_tiles) t -= p.t_tiles, ++gs;
+    }
+    __device__ __forceinline__ int group(const DensePairParams &p) const { return p.groups == 2 ? gs & 1 : 0; }
+    __device__ __forceinline__ int split(const DensePairParams &p) const { return p.groups == 2 ? gs >> 1 : gs; }
+    // reduction blocks [k0, k1) of the item
+    __device__ __forceinline__ void range(const DensePairParams &p, int &k0, int &k1) const {
+        k0 = 0, k1 = p.kb_total;
+        if (p.splits > 1) {
+            const int s = split(p);
+            k0 = (int)((long long)p.kb_total * s / p.splits), k1 = (int)((long long)p.kb_total * (s + 1) / p.splits);
+        }
+    }
+};
+
+// Epilogue of one warp: 32 rows x a quarter of the tile's columns (64, or 32 of a tile of 128), 16 columns at a time in ONE loop body.
 template <int MODE, int ACT>
-__device__ __forceinline__ void dense_pair_panel(const DensePairParams &p, const CUtensorMap *my, uint8_t *panel, uint64_t *res_bar, uint32_t res_phase,
-                                                 int *abort_flag, const float *bias, const float *bias2, uint32_t acc, uint32_t acc2, int c0, int row0,
-                                                 float *part) {
-    const int lane = threadIdx.x & 31;
+__device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, DensePairSmem &sm, const CUtensorMap *my, const CUtensorMap *mr,
+                                                    uint32_t tmem, uint32_t rank, DensePairTiles t) {
+    const int ew = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, q = ew & 3, g = ew >> 2;
+    const int f_width = MODE == DP_GATED ? p.bn / 2 : p.bn, width = f_width >> 2;  // 64 or 32
+    const int swz_shift = width == 64 ? 0 : 1, swz_mask = width == 64 ? 7 : 3;
     const int col_blocks = (p.F + 31) >> 5;
-    const bool rows_in = row0 < p.T;  // (warp-uniform; saved blocks and partial tiles exist for whole blocks of 32 rows)
-    if (MODE == DP_LINEAR && p.residual) {
-        if (p.tma_res) {
-            if (rows_in && c0 < p.F) mbar_wait_abortable(res_bar, res_phase, abort_flag);
-        } else {
-            for (int r = 0; r < 32; ++r) {  // any alignment: a row at a time, two columns per lane
-                const int t = row0 + r;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int c = h * 32 + lane;
-                    const unsigned short v = t < p.T && c0 + c < p.F ? p.residual[(long long)t * p.ld_res + c0 + c] : (unsigned short)0;
-                    *reinterpret_cast<unsigned short *>(panel + sw128_offset(r, c >> 3) + (c & 7) * 2) = v;
-                }
-            }
-            __syncwarp();
-        }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int c = c0 + h * 32;
-        float v[32];
-        load_run(acc + h * 32, v);
-        const bool live = rows_in && c < p.F;
-        if (MODE == DP_PARTIAL) {
-            if (live) save_run_f32(part, saved_block(row0, c, col_blocks), lane, v);
-            continue;
-        }
-        if (p.bias0) add_bias_run(v, bias + h * 32);
-        float u[32];
-        if (MODE == DP_GATED) {
-            load_run(acc2 + h * 32, u);
-            if (p.bias1) add_bias_run(u, bias2 + h * 32);
-        }
-        if (p.save0 && live) {
-            const size_t block = saved_block(row0, c, col_blocks);
-            if (p.save_f32) {
-                save_run_f32(reinterpret_cast<float *>(p.save0), block, lane, v);
-                if (MODE == DP_GATED) save_run_f32(reinterpret_cast<float *>(p.save1), block, lane, u);
-            } else {
-                save_run_f16(p.save0, p.save0 + p.save_scale_off, block, lane, v);
-                if (MODE == DP_GATED) save_run_f16(p.save1, p.save1 + p.save_scale_off, block, lane, u);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) act_pair<ACT>(v[i], v[i + 1]);
-        if (MODE == DP_GATED) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] *= u[i];
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            uint4 *at = reinterpret_cast<uint4 *>(panel + sw128_offset(lane, h * 4 + q));
-            if (MODE == DP_LINEAR && p.residual) {
-                const uint4 r = *at;
-                const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float lo, hi;
-                    unpack_bits16(w[i], p.half, lo, hi);
-                    v[q * 8 + 2 * i] += lo, v[q * 8 + 2 * i + 1] += hi;
-                }
-            }
-            *at = make_uint4(pack_bits16(v[q * 8], v[q * 8 + 1], p.half), pack_bits16(v[q * 8 + 2], v[q * 8 + 3], p.half),
-                             pack_bits16(v[q * 8 + 4], v[q * 8 + 5], p.half), pack_bits16(v[q * 8 + 6], v[q * 8 + 7], p.half));
-        }
-    }
-    if (MODE == DP_PARTIAL) return;
-    if (p.tma_out) {
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) {
-            if (rows_in && c0 < p.F) tma_store_2d(my, panel, c0, row0);
-            bulk_commit();
-        }
-    } else {
-        __syncwarp();
-        for (int r = 0; r < 32; ++r) {
-            const int t = row0 + r;
-            if (t >= p.T) break;
+    const uint32_t acc_free0 = map_to_rank(smem_u32(&sm.acc_free[0]), 0), acc_free1 = map_to_rank(smem_u32(&sm.acc_free[1]), 0);
+    uint8_t *panel = sm.panel[ew];
+    auto panel_at = [&](int row, int chunk) { return panel + row * (width * 2) + ((chunk ^ ((row >> swz_shift) & swz_mask)) << 4); };
+    const bool has_res = MODE == DP_LINEAR && p.residual != nullptr, has_bias = MODE != DP_PARTIAL && (p.bias0 || (MODE == DP_GATED && p.bias1));
+    uint32_t res_phase = 0;
+    for (int n = 0; t.valid(p); t.next(p), ++n) {
+        const int row0 = t.t * 256 + (int)rank * 128 + q * 32, col0 = t.f * f_width + g * width, a = n & 1;
+        const bool live = row0 < p.T && col0 < p.F;  // (warp-uniform)
+        // before the accumulator is ready: this lane's biases (columns lane, lane + 32 of the warp's run) and the residual's tile
+        float b0[2] = {0.f, 0.f}, b1[2] = {0.f, 0.f};
+        if (has_bias) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int c = h * 32 + lane;
-                if (c0 + c < p.F)
-                    p.out0[(long long)t * p.ld_out + c0 + c] = *reinterpret_cast<const unsigned short *>(panel + sw128_offset(r, c >> 3) + (c & 7) * 2);
+                if (c < width && col0 + c < p.F) {
+                    if (p.bias0) b0[h] = load_bias(p.bias0, col0 + c, p.bias_fp32, p.half);
+                    if (MODE == DP_GATED && p.bias1) b1[h] = load_bias(p.bias1, col0 + c, p.bias_fp32, p.half);
+                }
+            }
+        }
+        if (MODE != DP_PARTIAL && lane == 0) {
+            bulk_wait_read<0>();  // the panel's last store has been read out of shared memory
+            if (has_res && p.tma_res && live) {
+                fence_proxy_async();
+                mbar_expect_tx(&sm.res_full[ew], (uint32_t)width * 64);
+                tma_load_2d(panel, mr, col0, row0, &sm.res_full[ew]);
             }
         }
         __syncwarp();
-    }
-}
-
-struct DensePairTile {
-    int t0, f0, group, split, k0, k1;
-};
-__device__ __forceinline__ DensePairTile dense_pair_tile(const DensePairParams &p, int item, int f_width) {
-    DensePairTile t;
-    t.f0 = (item % p.f_tiles) * f_width;
-    item /= p.f_tiles;
-    t.t0 = (item % p.t_tiles) * 256;
-    item /= p.t_tiles;
-    t.group = item % p.groups;
-    t.split = item / p.groups;
-    t.k0 = (int)((long long)p.kb_total * t.split / p.splits);
-    t.k1 = (int)((long long)p.kb_total * (t.split + 1) / p.splits);
-    return t;
-}
-
-template <int MODE, int ACT>
-__device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, DensePairSmem &sm, const CUtensorMap *my, const CUtensorMap *mr,
-                                                    uint32_t tmem, uint32_t rank, int items, int pairs) {
-    const int warp = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, q = warp & 3, half = warp >> 2;
-    const int f_width = MODE == DP_GATED ? p.bn / 2 : p.bn;
-    const int panels = f_width / 128;  // 64-column panels of this warp: half the tile's columns
-    const uint32_t acc_free0 = map_to_rank(smem_u32(&sm.acc_free[0]), 0), acc_free1 = map_to_rank(smem_u32(&sm.acc_free[1]), 0);
-    int n = 0, used = 0;     // tiles done, panels done (the two staging buffers alternate)
-    uint32_t res_phase = 0;  // bit i: phase of res_full[i]
-    for (int item = blockIdx.x >> 1; item < items; item += pairs, ++n) {
-        const DensePairTile t = dense_pair_tile(p, item, f_width);
-        const int row0 = t.t0 + (int)rank * 128 + q * 32, col0 = t.f0 + half * panels * 64;
-        const int a = n & 1;
-        if (MODE != DP_PARTIAL && (p.bias0 || (MODE == DP_GATED && p.bias1))) {
-            const int i = threadIdx.x - 128;  // 0 .. 255: column of the accumulator
-            const void *b = MODE == DP_GATED && i >= f_width ? p.bias1 : p.bias0;
-            const int c = t.f0 + (MODE == DP_GATED && i >= f_width ? i - f_width : i);
-            sm.bias[a][i] = b && c < p.F && i < p.bn ? load_bias(b, c, p.bias_fp32, p.half) : 0.f;
-            asm volatile("bar.sync 1, 256;" ::: "memory");
-        }
-        if (MODE == DP_LINEAR && p.residual && p.tma_res && lane == 0) {
-            bulk_wait_read<0>();  // the panels' last stores have been read out of shared memory
-            fence_proxy_async();
-            for (int i = 0; i < panels; ++i)
-                if (row0 < p.T && col0 + i * 64 < p.F) {
-                    const int b = (used + i) & 1;
-                    mbar_expect_tx(&sm.res_full[warp][b], 4096);
-                    tma_load_2d(sm.panel[warp][b], mr, col0 + i * 64, row0, &sm.res_full[warp][b]);
+        if (has_res && !p.tma_res && live) {  // any alignment: a row at a time, a column per lane
+            for (int r = 0; r < 32; ++r)
+                for (int c = lane; c < width; c += 32) {
+                    const unsigned short v = row0 + r < p.T && col0 + c < p.F ? p.residual[(long long)(row0 + r) * p.ld_res + col0 + c] : (unsigned short)0;
+                    *reinterpret_cast<unsigned short *>(panel_at(r, c >> 3) + (c & 7) * 2) = v;
                 }
+            __syncwarp();
         }
-        __syncwarp();
-        const bool ok = mbar_wait_abortable(&sm.acc_full[a], (n >> 1) & 1, &sm.abort_flag);
-        if (!ok) break;
+        if (!mbar_wait_abortable(&sm.acc_full[a], (n >> 1) & 1, &sm.abort_flag)) break;
         tc_fence_after();
-        const uint32_t acc = tmem + a * 256 + ((uint32_t)(q * 32) << 16) + half * panels * 64;
-        float *part = MODE == DP_PARTIAL ? p.part + (size_t)(t.split * p.groups + t.group) * (saved_bytes_f32(p.T, p.F) / 4) : nullptr;
-        for (int i = 0; i < panels; ++i, ++used) {
-            const int b = used & 1;
-            if (MODE != DP_PARTIAL && !(MODE == DP_LINEAR && p.residual && p.tma_res)) {
-                if (lane == 0) bulk_wait_read<1>();  // this buffer's previous store has been read
+        if (live) {
+            // The four warps of a column group write the same biases to the same place.  Nobody still reads this buffer: the accumulator of tile n
+            // became full only after every warp had released tile n - 2.
+            float *bias = &sm.bias[a][g * width], *bias2 = &sm.bias[a][128 + g * width];
+            if (has_bias) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (h * 32 < width) {
+                        bias[h * 32 + lane] = b0[h];
+                        if (MODE == DP_GATED) bias2[h * 32 + lane] = b1[h];
+                    }
                 __syncwarp();
             }
-            dense_pair_panel<MODE, ACT>(p, my, sm.panel[warp][b], &sm.res_full[warp][b], (res_phase >> b) & 1, &sm.abort_flag,
-                                        &sm.bias[a][half * panels * 64 + i * 64], &sm.bias[a][(MODE == DP_GATED ? f_width : 0) + half * panels * 64 + i * 64],
-                                        acc + i * 64, acc + f_width + i * 64, col0 + i * 64, row0, part);
-            if (MODE == DP_LINEAR && p.residual && p.tma_res && row0 < p.T && col0 + i * 64 < p.F) res_phase ^= 1u << b;
+            if (has_res && p.tma_res) {
+                mbar_wait_abortable(&sm.res_full[ew], res_phase, &sm.abort_flag);
+                res_phase ^= 1;
+            }
+            const uint32_t acc = tmem + a * 256 + ((uint32_t)(q * 32) << 16) + g * width;
+            float *part = MODE == DP_PARTIAL ? p.part + (size_t)t.gs * (saved_bytes_f32(p.T, p.F) / 4) : nullptr;
+#pragma unroll 1
+            for (int c = 0; c < width; c += 16) {
+                const int col = col0 + c;
+                uint32_t raw[16], raw2[16];
+                tmem_ld16(acc + c, raw);
+                if (MODE == DP_GATED) tmem_ld16(acc + f_width + c, raw2);
+                tmem_wait_ld();
+                if (c + 16 == width) {  // the accumulator has been read: the products may have it back
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(a ? acc_free1 : acc_free0);
+                }
+                if (col >= p.F) continue;
+                float v[16], u[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    v[i] = __uint_as_float(raw[i]);
+                    if (MODE == DP_GATED) u[i] = __uint_as_float(raw2[i]);
+                }
+                const size_t block = saved_block(row0, col, col_blocks);
+                if (MODE == DP_PARTIAL) {
+                    save_run_f32(part, block, col, lane, v);
+                    continue;
+                }
+                if (has_bias) {
+                    add_bias_run(v, bias + c);
+                    if (MODE == DP_GATED) add_bias_run(u, bias2 + c);
+                }
+                if (p.save0) {
+                    if (p.save_f32) {
+                        save_run_f32(reinterpret_cast<float *>(p.save0), block, col, lane, v);
+                        if (MODE == DP_GATED) save_run_f32(reinterpret_cast<float *>(p.save1), block, col, lane, u);
+                    } else {
+                        save_run_f16(p.save0, p.save0 + p.save_exps, block, col, lane, v);
+                        if (MODE == DP_GATED) save_run_f16(p.save1, p.save1 + p.save_exps, block, col, lane, u);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) act_pair<ACT>(v[i], v[i + 1]);
+                if (MODE == DP_GATED) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) v[i] *= u[i];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    uint4 *at = reinterpret_cast<uint4 *>(panel_at(lane, (c >> 3) + h));
+                    if (has_res) {
+                        const uint4 r = *at;
+                        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float lo, hi;
+                            unpack_bits16(w[i], p.half, lo, hi);
+                            v[h * 8 + 2 * i] += lo, v[h * 8 + 2 * i + 1] += hi;
+                        }
+                    }
+                    *at = make_uint4(pack_bits16(v[h * 8], v[h * 8 + 1], p.half), pack_bits16(v[h * 8 + 2], v[h * 8 + 3], p.half),
+                                     pack_bits16(v[h * 8 + 4], v[h * 8 + 5], p.half), pack_bits16(v[h * 8 + 6], v[h * 8 + 7], p.half));
+                }
+            }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(a ? acc_free1 : acc_free0);
+        if (!live) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(a ? acc_free1 : acc_free0);
+        }
+        if (MODE == DP_PARTIAL || !live) continue;
+        if (p.tma_out) {
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                tma_store_2d(my, panel, col0, row0);
+                bulk_commit();
+            }
+        } else {
+            for (int r = 0; r < 32 && row0 + r < p.T; ++r)
+                for (int c = lane; c < width && col0 + c < p.F; c += 32)
+                    p.out0[(long long)(row0 + r) * p.ld_out + col0 + c] = *reinterpret_cast<const unsigned short *>(panel_at(r, c >> 3) + (c & 7) * 2);
+            __syncwarp();
+        }
     }
     if (lane == 0) bulk_wait_all();
     __syncwarp();
@@ -321,8 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
     }
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();
-    const int pairs = gridDim.x >> 1;
-    const int items = p.f_tiles * p.t_tiles * p.groups * p.splits;
+    DensePairTiles t(p, (int)blockIdx.x >> 1, (int)gridDim.x >> 1);
     const int f_width = MODE == DP_GATED ? p.bn / 2 : p.bn;
     const int b_rows = p.bn / 2;  // rows of B this CTA stages
 
@@ -335,8 +345,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.acc_full[i], 1);
             mbar_init(&sm.acc_free[i], 2 * DP_EPI_WARPS);
-            for (int w = 0; w < DP_EPI_WARPS; ++w) mbar_init(&sm.res_full[w][i], 1);
+            
         }
+        for (int w = 0; w < DP_EPI_WARPS; ++w) mbar_init(&sm.res_full[w], 1);
         sm.abort_flag = 0;
         mbar_fence_init();
     }
@@ -347,26 +358,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
 
+    // (The loops of warps 0 and 1 are run by the whole warp, one elected thread issuing: control flow and descriptors stay warp-uniform, which keeps
+    // the instructions between two products few.  Run by one thread alone they took 620 cycles per reduction block, and 1200 beside a busy
+    // epilogue, where the products themselves take 512.)
     if (warp == 0) {
-        if (lane == 0) {
-            int slot = 0;
-            uint32_t phase = 0;
-            bool ok = true;
-            for (int item = blockIdx.x >> 1; item < items && ok; item += pairs) {
-                const DensePairTile t = dense_pair_tile(p, item, f_width);
-                const int ta = t.t0 + (int)rank * 128;
-                const int fb = MODE == DP_GATED ? t.f0 : t.f0 + (int)rank * b_rows;
-                for (int kb = t.k0; kb < t.k1; ++kb) {
-                    if (!mbar_wait_abortable(&sm.free[slot], phase ^ 1, &sm.abort_flag)) {
-                        ok = false;
-                        break;
-                    }
+        const bool leader = elect_one();
+        int slot = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        const uint32_t bytes = 2 * (16384 + (uint32_t)b_rows * 128), full0 = map_to_rank(smem_u32(&sm.full[0]), 0);
+        for (; t.valid(p) && ok; t.next(p)) {
+            const int ta = t.t * 256 + (int)rank * 128, fb = t.f * f_width + (MODE == DP_GATED ? 0 : (int)rank * b_rows), group = t.group(p);
+            int k0, k1;
+            t.range(p, k0, k1);
+            for (int kb = k0; kb < k1; ++kb) {
+                if (!mbar_wait_abortable(&sm.free[slot], phase ^ 1, &sm.abort_flag)) {
+                    ok = false;
+                    break;
+                }
+                if (leader) {
                     uint8_t *a = sm.stage[slot], *b = a + 16384;
-                    if (rank == 0) mbar_expect_tx(&sm.full[slot], 2 * (16384 + (uint32_t)b_rows * 128));
-                    const uint32_t bar = map_to_rank(smem_u32(&sm.full[slot]), 0);
+                    if (rank == 0) mbar_expect_tx(&sm.full[slot], bytes);
+                    const uint32_t bar = full0 + slot * 8;
                     const bool second = kb >= p.kb_seg;
                     const int r = (second ? kb - p.kb_seg : kb) * DT_BK;
-                    const CUtensorMap *mA = (second || t.group) ? &ma1 : &ma0;
+                    const CUtensorMap *mA = (second || group) ? &ma1 : &ma0;
                     const CUtensorMap *mB = (second || (MODE == DP_GATED && rank)) ? &mb1 : &mb0;
                     if (p.a_mn) {
                         tma_load_2d_pair(a, mA, ta, r, bar);
@@ -379,50 +395,55 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
                     } else {
                         tma_load_2d_pair(b, mB, r, fb, bar);
                     }
-                    if (++slot == DP_STAGES) slot = 0, phase ^= 1;
                 }
+                __syncwarp();
+                if (++slot == DP_STAGES) slot = 0, phase ^= 1;
             }
         }
-        __syncwarp();
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
+            const bool leader = elect_one();
             const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
             const uint64_t ad0 = umma_desc_sw128(smem_u32(sm.stage[0]), p.a_mn ? 8192 : 16, 1024);
             const uint64_t bd0 = umma_desc_sw128(smem_u32(sm.stage[0]) + 16384, p.b_mn ? 8192 : 16, 1024);
-            int slot = 0, n = 0;
+            int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int item = blockIdx.x >> 1; item < items && ok; item += pairs, ++n) {
-                const DensePairTile t = dense_pair_tile(p, item, f_width);
+            for (int n = 0; t.valid(p) && ok; t.next(p), ++n) {
                 const int acc = n & 1;
+                int k0, k1;
+                t.range(p, k0, k1);
                 if (!mbar_wait_abortable(&sm.acc_free[acc], ((n >> 1) & 1) ^ 1, &sm.abort_flag)) break;
                 tc_fence_after();
-                for (int kb = t.k0; kb < t.k1; ++kb) {
+                for (int kb = k0; kb < k1; ++kb) {
                     if (!mbar_wait_abortable(&sm.full[slot], phase, &sm.abort_flag)) {
                         ok = false;
                         break;
                     }
                     tc_fence_after();
-                    const uint64_t ad = ad0 + (uint64_t)slot * (DP_STAGE_BYTES >> 4), bd = bd0 + (uint64_t)slot * (DP_STAGE_BYTES >> 4);
+                    if (leader) {
+                        const uint64_t ad = ad0 + (uint64_t)(slot * (DP_STAGE_BYTES >> 4)), bd = bd0 + (uint64_t)(slot * (DP_STAGE_BYTES >> 4));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) umma_ss_pair(tmem + acc * 256, ad + k * a_step, bd + k * b_step, p.idesc, kb > t.k0 || k > 0);
-                    umma_commit_pair(&sm.free[slot]);
+                        for (int k = 0; k < 4; ++k) umma_ss_pair(tmem + acc * 256, ad + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
+                        umma_commit_pair(&sm.free[slot]);
+                    }
+                    __syncwarp();
                     if (++slot == DP_STAGES) slot = 0, phase ^= 1;
                 }
-                if (ok) umma_commit_pair(&sm.acc_full[acc]);
+                if (ok && leader) umma_commit_pair(&sm.acc_full[acc]);
+                __syncwarp();
             }
         }
-        __syncwarp();
     } else if (warp >= 4) {
         if (MODE == DP_PARTIAL) {
-            dense_pair_epilogue<MODE, ACT_NONE>(p, sm, &my, &mr, tmem, rank, items, pairs);
+            dense_pair_epilogue<MODE, ACT_NONE>(p, sm, &my, &mr, tmem, rank, t);
         } else {
             switch (p.act) {
-                case ACT_GELU: dense_pair_epilogue<MODE, ACT_GELU>(p, sm, &my, &mr, tmem, rank, items, pairs); break;
-                case ACT_SILU: dense_pair_epilogue<MODE, ACT_SILU>(p, sm, &my, &mr, tmem, rank, items, pairs); break;
-                case ACT_RELU: dense_pair_epilogue<MODE, ACT_RELU>(p, sm, &my, &mr, tmem, rank, items, pairs); break;
-                case ACT_SIGMOID: dense_pair_epilogue<MODE, ACT_SIGMOID>(p, sm, &my, &mr, tmem, rank, items, pairs); break;
-                default: dense_pair_epilogue<MODE, ACT_NONE>(p, sm, &my, &mr, tmem, rank, items, pairs);
+                case ACT_GELU: dense_pair_epilogue<MODE, ACT_GELU>(p, sm, &my, &mr, tmem, rank, t); break;
+                case ACT_SILU: dense_pair_epilogue<MODE, ACT_SILU>(p, sm, &my, &mr, tmem, rank, t); break;
+                case ACT_RELU: dense_pair_epilogue<MODE, ACT_RELU>(p, sm, &my, &mr, tmem, rank, t); break;
+                case ACT_SIGMOID: dense_pair_epilogue<MODE, ACT_SIGMOID>(p, sm, &my, &mr, tmem, rank, t); break;
+                default: dense_pair_epilogue<MODE, ACT_NONE>(p, sm, &my, &mr, tmem, rank, t);
             }
         }
     }
