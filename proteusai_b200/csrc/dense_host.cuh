@@ -230,10 +230,10 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     const bool partial = c.splits > 1;
     p.tma_out = !partial && ((uintptr_t)d.out[0] & 15) == 0 && (d.T == 1 || (d.ld_out & 7) == 0);
     if (p.tma_out)
-        if (int e = make_map_16(&m[4], d.out[0], d.F, d.T, d.ld_out, 32, d.half, fw / 4)) return e;
+        if (int e = make_map_16(&m[4], d.out[0], d.F, d.T, d.ld_out, 32, d.half, 32)) return e;
     p.tma_res = d.residual && ((uintptr_t)d.residual & 15) == 0 && (d.T == 1 || ((d.ld_res & 7) == 0 && d.ld_res >= d.F));
     if (p.tma_res)
-        if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half, fw / 4)) return e;
+        if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half, 32)) return e;
     const int ctas = 2 * (int)(items < sms / 2 ? items : sms / 2);
     if (partial) {
         if (int e = dense_pair_launch_as<DP_PARTIAL>(m, p, ctas, st)) return e;

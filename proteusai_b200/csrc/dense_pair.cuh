@@ -5,7 +5,7 @@
 // epilogue of one tile runs under the products of the next.
 //
 // An accumulator lane is an output ROW here (the operands of dense_tile.cuh swapped): a thread of the epilogue holds runs of 32 columns, packs
-// them to 16-byte words, and the tile leaves through shared memory by TMA stores (64 columns x 32 rows per warp and step).
+// them to 16-byte words, and the tile leaves through shared memory by TMA stores (32 columns x 32 rows per warp and step).
 //     forward  t = token,           f = output feature, r = input feature:  A = x  (K-major),  B = W (K-major)
 //     gated    the same with B = 128 rows of Wg (staged by the pair's first CTA) and 128 of Wu (by its second): columns [0, 128) of the
 //              accumulator are g, [128, 256) are u
@@ -28,10 +28,10 @@ constexpr int DP_EPI_WARPS = 16;
 
 struct DensePairSmem {
     uint8_t stage[DP_STAGES][DP_STAGE_BYTES];
-    uint8_t panel[DP_EPI_WARPS][4096];  // per epilogue warp: 32 rows x 64 (128-byte swizzle) or 32 columns (64-byte swizzle); output and residual
+    uint8_t panel[DP_EPI_WARPS][2][2048];  // per epilogue warp two of 32 rows x 32 columns (64-byte swizzle): residual in, output out
     float bias[2][256];
     uint64_t full[DP_STAGES], free[DP_STAGES], acc_full[2], acc_free[2];
-    uint64_t res_full[DP_EPI_WARPS];
+    uint64_t res_full[DP_EPI_WARPS][2];
     uint32_t tmem;
     int abort_flag;
 };
@@ -64,6 +64,8 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
     return r;
 }
+// Byte offset of the 16-byte chunk `chunk` (0..3) of row `row` inside a [rows x 64 B] tile stored with the 64-byte swizzle.
+__device__ __forceinline__ uint32_t sw64_offset(int row, int chunk) { return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); }
 // one thread of a converged warp
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;
@@ -168,152 +170,191 @@ struct DensePairTiles {
     }
 };
 
-// Epilogue of one warp: 32 rows x a quarter of the tile's columns (64, or 32 of a tile of 128), 16 columns at a time in ONE loop body.
+// The 16 columns from `c` of a 32-column panel: bias, saved pre-activations, activation, product, residual, rounding, into the panel.
+template <int MODE, int ACT>
+__device__ __forceinline__ void dense_pair_run(const DensePairParams &p, const uint32_t *raw, const uint32_t *raw2, const float *bias, const float *bias2,
+                                               bool has_bias, bool has_res, uint8_t *panel, int c, int col, size_t block) {
+    const int lane = threadIdx.x & 31;
+    float v[16], u[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        v[i] = __uint_as_float(raw[i]);
+        if (MODE == DP_GATED) u[i] = __uint_as_float(raw2[i]);
+    }
+    if (has_bias) {
+        add_bias_run(v, bias + c);
+        if (MODE == DP_GATED) add_bias_run(u, bias2 + c);
+    }
+    if (p.save0) {
+        if (p.save_f32) {
+            save_run_f32(reinterpret_cast<float *>(p.save0), block, col, lane, v);
+            if (MODE == DP_GATED) save_run_f32(reinterpret_cast<float *>(p.save1), block, col, lane, u);
+        } else {
+            save_run_f16(p.save0, p.save0 + p.save_exps, block, col, lane, v);
+            if (MODE == DP_GATED) save_run_f16(p.save1, p.save1 + p.save_exps, block, col, lane, u);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i += 2) act_pair<ACT>(v[i], v[i + 1]);
+    if (MODE == DP_GATED) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= u[i];
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        uint4 *at = reinterpret_cast<uint4 *>(panel + sw64_offset(lane, (c >> 3) + h));
+        if (has_res) {
+            const uint4 r = *at;
+            const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float lo, hi;
+                unpack_bits16(w[i], p.half, lo, hi);
+                v[h * 8 + 2 * i] += lo, v[h * 8 + 2 * i + 1] += hi;
+            }
+        }
+        *at = make_uint4(pack_bits16(v[h * 8], v[h * 8 + 1], p.half), pack_bits16(v[h * 8 + 2], v[h * 8 + 3], p.half),
+                         pack_bits16(v[h * 8 + 4], v[h * 8 + 5], p.half), pack_bits16(v[h * 8 + 6], v[h * 8 + 7], p.half));
+    }
+}
+
+// Epilogue of one warp: 32 rows x a quarter of the tile's columns, in panels of 32 columns that alternate between two buffers: while one is
+// computed the other leaves by its TMA store, and the residual of the next panel is on its way into it as soon as that store has read it.
 template <int MODE, int ACT>
 __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, DensePairSmem &sm, const CUtensorMap *my, const CUtensorMap *mr,
                                                     uint32_t tmem, uint32_t rank, DensePairTiles t) {
     const int ew = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, q = ew & 3, g = ew >> 2;
-    const int f_width = MODE == DP_GATED ? p.bn / 2 : p.bn, width = f_width >> 2;  // 64 or 32
-    const int swz_shift = width == 64 ? 0 : 1, swz_mask = width == 64 ? 7 : 3;
+    const int f_width = MODE == DP_GATED ? p.bn / 2 : p.bn, panels = f_width >> 7;  // panels of this warp per tile: 2 or 1
     const int col_blocks = (p.F + 31) >> 5;
     const uint32_t acc_free0 = map_to_rank(smem_u32(&sm.acc_free[0]), 0), acc_free1 = map_to_rank(smem_u32(&sm.acc_free[1]), 0);
-    uint8_t *panel = sm.panel[ew];
-    auto panel_at = [&](int row, int chunk) { return panel + row * (width * 2) + ((chunk ^ ((row >> swz_shift) & swz_mask)) << 4); };
-    const bool has_res = MODE == DP_LINEAR && p.residual != nullptr, has_bias = MODE != DP_PARTIAL && (p.bias0 || (MODE == DP_GATED && p.bias1));
-    uint32_t res_phase = 0;
-    for (int n = 0; t.valid(p); t.next(p), ++n) {
-        const int row0 = t.t * 256 + (int)rank * 128 + q * 32, col0 = t.f * f_width + g * width, a = n & 1;
-        const bool live = row0 < p.T && col0 < p.F;  // (warp-uniform)
-        // before the accumulator is ready: this lane's biases (columns lane, lane + 32 of the warp's run) and the residual's tile
-        float b0[2] = {0.f, 0.f}, b1[2] = {0.f, 0.f};
-        if (has_bias) {
+    const bool has_res = MODE == DP_LINEAR && p.residual != nullptr, res_tma = has_res && p.tma_res;
+    const bool has_bias = MODE != DP_PARTIAL && (p.bias0 || (MODE == DP_GATED && p.bias1));
+    auto row_of = [&](const DensePairTiles &x) { return x.t * 256 + (int)rank * 128 + q * 32; };
+    auto col_of = [&](const DensePairTiles &x, int i) { return x.f * f_width + (g * panels + i) * 32; };
+    auto fetch_residual = [&](const DensePairTiles &x, int i, int b) {  // (one lane)
+        if (row_of(x) < p.T && col_of(x, i) < p.F) {
+            mbar_expect_tx(&sm.res_full[ew][b], 2048);
+            tma_load_2d(sm.panel[ew][b], mr, col_of(x, i), row_of(x), &sm.res_full[ew][b]);
+        }
+    };
+    float b0[2], b1[2];  // this lane's biases (column lane of each panel), fetched a tile ahead
+    auto fetch_biases = [&](const DensePairTiles &x) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int c = h * 32 + lane;
-                if (c < width && col0 + c < p.F) {
-                    if (p.bias0) b0[h] = load_bias(p.bias0, col0 + c, p.bias_fp32, p.half);
-                    if (MODE == DP_GATED && p.bias1) b1[h] = load_bias(p.bias1, col0 + c, p.bias_fp32, p.half);
-                }
-            }
+        for (int i = 0; i < 2; ++i) {
+            const int c = col_of(x, i) + lane;
+            const bool in = i < panels && c < p.F;
+            b0[i] = in && p.bias0 ? load_bias(p.bias0, c, p.bias_fp32, p.half) : 0.f;
+            if (MODE == DP_GATED) b1[i] = in && p.bias1 ? load_bias(p.bias1, c, p.bias_fp32, p.half) : 0.f;
         }
-        if (MODE != DP_PARTIAL && lane == 0) {
-            bulk_wait_read<0>();  // the panel's last store has been read out of shared memory
-            if (has_res && p.tma_res && live) {
-                fence_proxy_async();
-                mbar_expect_tx(&sm.res_full[ew], (uint32_t)width * 64);
-                tma_load_2d(panel, mr, col0, row0, &sm.res_full[ew]);
-            }
-        }
-        __syncwarp();
-        if (has_res && !p.tma_res && live) {  // any alignment: a row at a time, a column per lane
-            for (int r = 0; r < 32; ++r)
-                for (int c = lane; c < width; c += 32) {
-                    const unsigned short v = row0 + r < p.T && col0 + c < p.F ? p.residual[(long long)(row0 + r) * p.ld_res + col0 + c] : (unsigned short)0;
-                    *reinterpret_cast<unsigned short *>(panel_at(r, c >> 3) + (c & 7) * 2) = v;
-                }
-            __syncwarp();
-        }
+    };
+    if (has_bias) fetch_biases(t);
+    if (res_tma && lane == 0) fetch_residual(t, 0, 0);
+    uint32_t res_phase = 0;  // bit b: phase of res_full[b]
+    int used = 0;            // panels so far
+    for (int n = 0; t.valid(p); ++n) {
+        const int row0 = row_of(t), a = n & 1;
+        DensePairTiles next = t;
+        next.next(p);
         if (!mbar_wait_abortable(&sm.acc_full[a], (n >> 1) & 1, &sm.abort_flag)) break;
         tc_fence_after();
-        if (live) {
-            // The four warps of a column group write the same biases to the same place.  Nobody still reads this buffer: the accumulator of tile n
-            // became full only after every warp had released tile n - 2.
-            float *bias = &sm.bias[a][g * width], *bias2 = &sm.bias[a][128 + g * width];
-            if (has_bias) {
+        // The four warps of a column group write the same biases to the same place.  Nobody still reads this buffer: the accumulator of tile n
+        // became full only after every warp had released tile n - 2.
+        float *bias = &sm.bias[a][g * panels * 32], *bias2 = &sm.bias[a][128 + g * 32];
+        if (has_bias) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (h * 32 < width) {
-                        bias[h * 32 + lane] = b0[h];
-                        if (MODE == DP_GATED) bias2[h * 32 + lane] = b1[h];
-                    }
+            for (int i = 0; i < 2; ++i)
+                if (i < panels) {
+                    bias[i * 32 + lane] = b0[i];
+                    if (MODE == DP_GATED) bias2[lane] = b1[0];
+                }
+            if (next.valid(p)) fetch_biases(next);
+            __syncwarp();
+        }
+        const uint32_t acc = tmem + a * 256 + ((uint32_t)(q * 32) << 16) + g * panels * 32;
+#pragma unroll 1
+        for (int i = 0; i < panels; ++i, ++used) {
+            const int col = col_of(t, i), b = used & 1;
+            const bool live = row0 < p.T && col < p.F, last = i + 1 == panels;  // (warp-uniform)
+            uint8_t *panel = sm.panel[ew][b];
+            if (MODE != DP_PARTIAL && !res_tma) {
+                if (lane == 0) bulk_wait_read<1>();  // the store before the last one has read this buffer
                 __syncwarp();
             }
-            if (has_res && p.tma_res) {
-                mbar_wait_abortable(&sm.res_full[ew], res_phase, &sm.abort_flag);
-                res_phase ^= 1;
+            if (has_res && !p.tma_res && live) {  // any alignment: a row at a time, a column per lane
+#pragma unroll 4
+                for (int r = 0; r < 32; ++r) {
+                    const unsigned short v = row0 + r < p.T && col + lane < p.F ? p.residual[(long long)(row0 + r) * p.ld_res + col + lane] : (unsigned short)0;
+                    *reinterpret_cast<unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2) = v;
+                }
+                __syncwarp();
             }
-            const uint32_t acc = tmem + a * 256 + ((uint32_t)(q * 32) << 16) + g * width;
-            float *part = MODE == DP_PARTIAL ? p.part + (size_t)t.gs * (saved_bytes_f32(p.T, p.F) / 4) : nullptr;
+            const size_t block = saved_block(row0, col, col_blocks);
+            auto release = [&]() {  // the accumulator has been read: the products may have it back
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(a ? acc_free1 : acc_free0);
+            };
+            if (MODE == DP_GATED) {
 #pragma unroll 1
-            for (int c = 0; c < width; c += 16) {
-                const int col = col0 + c;
-                uint32_t raw[16], raw2[16];
-                tmem_ld16(acc + c, raw);
-                if (MODE == DP_GATED) tmem_ld16(acc + f_width + c, raw2);
+                for (int c = 0; c < 32; c += 16) {
+                    uint32_t raw[16], raw2[16];
+                    tmem_ld16(acc + c, raw);
+                    tmem_ld16(acc + f_width + c, raw2);
+                    tmem_wait_ld();
+                    if (c == 16) release();
+                    if (live) dense_pair_run<MODE, ACT>(p, raw, raw2, bias, bias2, has_bias, false, panel, c, col + c, block);
+                }
+            } else {
+                uint32_t raw[32];
+                tmem_ld32(acc + i * 32, raw);
                 tmem_wait_ld();
-                if (c + 16 == width) {  // the accumulator has been read: the products may have it back
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(a ? acc_free1 : acc_free0);
+                if (last) release();
+                if (live && res_tma) {
+                    mbar_wait_abortable(&sm.res_full[ew][b], (res_phase >> b) & 1, &sm.abort_flag);
+                    res_phase ^= 1u << b;
                 }
-                if (col >= p.F) continue;
-                float v[16], u[16];
+                if (live) {
+                    if (MODE == DP_PARTIAL) {
+                        float *part = p.part + (size_t)t.gs * (saved_bytes_f32(p.T, p.F) / 4);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    v[i] = __uint_as_float(raw[i]);
-                    if (MODE == DP_GATED) u[i] = __uint_as_float(raw2[i]);
-                }
-                const size_t block = saved_block(row0, col, col_blocks);
-                if (MODE == DP_PARTIAL) {
-                    save_run_f32(part, block, col, lane, v);
-                    continue;
-                }
-                if (has_bias) {
-                    add_bias_run(v, bias + c);
-                    if (MODE == DP_GATED) add_bias_run(u, bias2 + c);
-                }
-                if (p.save0) {
-                    if (p.save_f32) {
-                        save_run_f32(reinterpret_cast<float *>(p.save0), block, col, lane, v);
-                        if (MODE == DP_GATED) save_run_f32(reinterpret_cast<float *>(p.save1), block, col, lane, u);
-                    } else {
-                        save_run_f16(p.save0, p.save0 + p.save_exps, block, col, lane, v);
-                        if (MODE == DP_GATED) save_run_f16(p.save1, p.save1 + p.save_exps, block, col, lane, u);
-                    }
-                }
+                        for (int c = 0; c < 32; c += 16) {
+                            float v[16];
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) act_pair<ACT>(v[i], v[i + 1]);
-                if (MODE == DP_GATED) {
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) v[i] *= u[i];
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint4 *at = reinterpret_cast<uint4 *>(panel_at(lane, (c >> 3) + h));
-                    if (has_res) {
-                        const uint4 r = *at;
-                        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float lo, hi;
-                            unpack_bits16(w[i], p.half, lo, hi);
-                            v[h * 8 + 2 * i] += lo, v[h * 8 + 2 * i + 1] += hi;
+                            for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(raw[c + k]);
+                            save_run_f32(part, block, c, lane, v);
                         }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 16)
+                            dense_pair_run<MODE, ACT>(p, raw + c, nullptr, bias + i * 32, nullptr, has_bias, has_res, panel, c, col + c, block);
                     }
-                    *at = make_uint4(pack_bits16(v[h * 8], v[h * 8 + 1], p.half), pack_bits16(v[h * 8 + 2], v[h * 8 + 3], p.half),
-                                     pack_bits16(v[h * 8 + 4], v[h * 8 + 5], p.half), pack_bits16(v[h * 8 + 6], v[h * 8 + 7], p.half));
                 }
             }
-        }
-        if (!live) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(a ? acc_free1 : acc_free0);
-        }
-        if (MODE == DP_PARTIAL || !live) continue;
-        if (p.tma_out) {
-            fence_proxy_async();
-            __syncwarp();
-            if (lane == 0) {
-                tma_store_2d(my, panel, col0, row0);
-                bulk_commit();
+            if (MODE == DP_PARTIAL) continue;
+            if (p.tma_out) {
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    if (live) tma_store_2d(my, panel, col, row0);
+                    bulk_commit();
+                }
+            } else if (live) {
+                __syncwarp();
+#pragma unroll 4
+                for (int r = 0; r < 32; ++r)
+                    if (row0 + r < p.T && col + lane < p.F)
+                        p.out0[(long long)(row0 + r) * p.ld_out + col + lane] = *reinterpret_cast<const unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2);
+                __syncwarp();
             }
-        } else {
-            for (int r = 0; r < 32 && row0 + r < p.T; ++r)
-                for (int c = lane; c < width && col0 + c < p.F; c += 32)
-                    p.out0[(long long)(row0 + r) * p.ld_out + col0 + c] = *reinterpret_cast<const unsigned short *>(panel_at(r, c >> 3) + (c & 7) * 2);
+            if (res_tma && lane == 0) {  // the next panel's residual into the other buffer, once the store before this one has read it
+                bulk_wait_read<1>();
+                fence_proxy_async();
+                if (!last) fetch_residual(t, i + 1, b ^ 1);
+                else if (next.valid(p)) fetch_residual(next, 0, b ^ 1);
+            }
             __syncwarp();
         }
+        t = next;
     }
     if (lane == 0) bulk_wait_all();
     __syncwarp();
@@ -347,7 +388,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
             mbar_init(&sm.acc_free[i], 2 * DP_EPI_WARPS);
             
         }
-        for (int w = 0; w < DP_EPI_WARPS; ++w) mbar_init(&sm.res_full[w], 1);
+        for (int w = 0; w < 2 * DP_EPI_WARPS; ++w) mbar_init(&sm.res_full[0][0] + w, 1);
         sm.abort_flag = 0;
         mbar_fence_init();
     }
