@@ -176,17 +176,17 @@ static int make_operand_map(CUtensorMap *m, const DenseOperand &o, int mn, long 
     return mn ? make_map_16(m, o.p, rows, R, o.ld, 64, half) : make_map_16(m, o.p, R, rows, o.ld, box, half);
 }
 
-template <int MODE>
+template <int MODE, int HALF>
 static int dense_pair_launch_as(const CUtensorMap (&m)[6], const DensePairParams &p, int ctas, cudaStream_t st) {
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel<MODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DensePairSmem));
+        cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel<MODE, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DensePairSmem));
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    dense_pair_kernel<MODE><<<ctas, DP_THREADS, sizeof(DensePairSmem), st>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
+    dense_pair_kernel<MODE, HALF><<<ctas, DP_THREADS, sizeof(DensePairSmem), st>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
     return (int)cudaPeekAtLastError();
 }
 
@@ -215,7 +215,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     p.T = (int)d.T, p.F = (int)d.F, p.bn = c.width;
     p.t_tiles = (int)((d.T + 255) / 256), p.f_tiles = (int)((d.F + fw - 1) / fw), p.groups = d.groups, p.splits = c.splits;
     p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
-    p.a_mn = d.b_mn, p.b_mn = d.a_mn, p.act = d.act, p.half = d.half;
+    p.a_mn = d.b_mn, p.b_mn = d.a_mn, p.act = d.act;
     p.idesc = dense_idesc(256, c.width, d, d.b_mn, d.a_mn);
     const long long items = (long long)p.t_tiles * p.f_tiles * p.groups * p.splits;
     if (items > 0x3fffffffll) return (int)PAI_ERR_BAD_SHAPE;
@@ -236,13 +236,14 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
         if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half, 32)) return e;
     const int ctas = 2 * (int)(items < sms / 2 ? items : sms / 2);
     if (partial) {
-        if (int e = dense_pair_launch_as<DP_PARTIAL>(m, p, ctas, st)) return e;
+        if (int e = dense_pair_launch_as<DP_PARTIAL, 0>(m, p, ctas, st)) return e;
         const size_t blocks = saved_blocks(d.T, (int)d.F);
         dense_reduce_kernel<<<dim3((unsigned)((blocks + 7) / 8), d.groups), 256, 0, st>>>(d.part, (unsigned short *)d.out[0], (unsigned short *)d.out[1],
                                                                                         p.T, p.F, d.ld_out, d.groups, c.splits, d.half);
         return (int)cudaPeekAtLastError();
     }
-    return d.dual ? dense_pair_launch_as<DP_GATED>(m, p, ctas, st) : dense_pair_launch_as<DP_LINEAR>(m, p, ctas, st);
+    if (d.half) return d.dual ? dense_pair_launch_as<DP_GATED, 1>(m, p, ctas, st) : dense_pair_launch_as<DP_LINEAR, 1>(m, p, ctas, st);
+    return d.dual ? dense_pair_launch_as<DP_GATED, 0>(m, p, ctas, st) : dense_pair_launch_as<DP_LINEAR, 0>(m, p, ctas, st);
 }
 
 static int dense_launch(const DenseProduct &d, int sms, cudaStream_t st) {

@@ -23,39 +23,39 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return y;
 }
 
-// log2 Phi(-a), a >= 0, as a polynomial of degree 7: Chebyshev fit of log2 of the normal distribution function on [0, 6], so that
-// 2^p has a RELATIVE error below 4e-6 there (half a bf16 step is 2^-9 .. 2^-8, half an fp16 step 2^-12 .. 2^-11).  Beyond 6 it keeps
-// falling (its leading coefficient is negative), where x Phi(x) is below 1e-8 in magnitude: the absolute error of x Phi(x) stays
-// below 6e-7 on the whole negative axis.  One SFU operation, against two for the rational form of erfc.  a is cut off at 30, where
-// Phi(-a) is 0 in fp32, so that infinities do not meet that 0.
+// log2 Phi(n), n <= 0, as a polynomial of degree 7: Chebyshev fit of log2 of the normal distribution function on [-6, 0], so that
+// 2^p has a RELATIVE error below 4e-6 there (half a bf16 step is 2^-9 .. 2^-8, half an fp16 step 2^-12 .. 2^-11).  Below -6 it keeps
+// falling, where x Phi(x) is below 1e-8 in magnitude: the absolute error of x Phi(x) stays
+// below 6e-7 on the whole negative axis.  One SFU operation, against two for the rational form of erfc.  n is cut off at -30, where
+// Phi(n) is 0 in fp32, so that infinities do not meet that 0.
 #define PAI_PHI_COEFFS                                                                                                    \
-    {-9.999943403e-01f, -1.151269147e+00f, -4.584097768e-01f, -5.402068712e-02f, 8.539461332e-03f, -9.388679333e-04f, \
-     6.268140101e-05f,  -1.889626234e-06f}
+    {-9.999943403e-01f, 1.151269147e+00f, -4.584097768e-01f, 5.402068712e-02f, 8.539461332e-03f, 9.388679333e-04f, \
+     6.268140101e-05f,  1.889626234e-06f}
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
-// Phi(-min(|x|, 30))
-__device__ __forceinline__ float normal_tail(float a) {
+// Phi(n) for n in [-30, 0]
+__device__ __forceinline__ float normal_tail(float n) {
     constexpr float c[8] = PAI_PHI_COEFFS;
     float p = c[7];
 #pragma unroll
-    for (int i = 6; i >= 0; --i) p = fmaf(p, a, c[i]);
+    for (int i = 6; i >= 0; --i) p = fmaf(p, n, c[i]);
     return ex2_approx(p);
 }
-// x Phi(x) = max(x, 0) - |x| Phi(-|x|) for a pair, the polynomial in packed arithmetic
+// x Phi(x) = max(x, 0) + n Phi(n), n = -min(|x|, 30), for a pair, the polynomial in packed arithmetic
 __device__ __forceinline__ void gelu2(float &x0, float &x1) {
     constexpr float c[8] = PAI_PHI_COEFFS;
-    const f2_t a = f2_pack(fminf(fabsf(x0), 30.f), fminf(fabsf(x1), 30.f));
+    const f2_t n = f2_pack(fmaxf(-fabsf(x0), -30.f), fmaxf(-fabsf(x1), -30.f));
     f2_t p = f2_pack(c[7], c[7]);
 #pragma unroll
-    for (int i = 6; i >= 0; --i) p = f2_fma(p, a, f2_pack(c[i], c[i]));
+    for (int i = 6; i >= 0; --i) p = f2_fma(p, n, f2_pack(c[i], c[i]));
     float p0, p1;
     f2_unpack(p, p0, p1);
-    const f2_t e = f2_pack(-ex2_approx(p0), -ex2_approx(p1));
-    f2_unpack(f2_fma(a, e, f2_pack(max_nan(x0, 0.f), max_nan(x1, 0.f))), x0, x1);
+    const f2_t e = f2_pack(ex2_approx(p0), ex2_approx(p1));
+    f2_unpack(f2_fma(n, e, f2_pack(max_nan(x0, 0.f), max_nan(x1, 0.f))), x0, x1);
 }
 __device__ __forceinline__ float sigmoid_f(float x) { return rcp_approx(1.f + ex2_approx(-1.4426950408889634f * x)); }
 
@@ -76,8 +76,8 @@ __device__ __forceinline__ void act_pair(float &a, float &b) {
 __device__ __forceinline__ void act_and_slope(int act, float z, float &a, float &d) {
     switch (act) {
         case ACT_GELU: {
-            const float t = fminf(fabsf(z), 30.f), e = normal_tail(t), phi = z < 0.f ? e : 1.f - e;
-            a = fmaf(-t, e, max_nan(z, 0.f));
+            const float n = fmaxf(-fabsf(z), -30.f), e = normal_tail(n), phi = z < 0.f ? e : 1.f - e;
+            a = fmaf(n, e, max_nan(z, 0.f));
             d = fmaf(z * 0.3989422804014327f, ex2_approx(-0.7213475204444817f * z * z), phi);
             break;
         }

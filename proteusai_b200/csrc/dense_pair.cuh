@@ -13,18 +13,16 @@
 //     dW       t = output feature,  f = input feature,  r = token:          A = dz (MN-major), B = x (MN-major); the long reduction split
 //              over pairs that leave fp32 tiles in the workspace, added in order by dense_reduce_kernel
 //
-// Warps: 0 TMA loads, 1 MMAs (first CTA of the pair), 2 tensor memory, 4..19 epilogue (four per quarter of the lanes, a quarter of the
-// columns each: the epilogue is a chain of latencies, and with eight warps and a barrier per tile it took three times as long as the products
-// of a short reduction).
+// Warps: 0 TMA loads, 1 MMAs (first CTA of the pair), 2 tensor memory, 4..11 epilogue (two per quarter of the lanes, half the columns each).
 #pragma once
 #include "dense_tile.cuh"
 
 namespace pai {
 
-constexpr int DP_THREADS = 640;
 constexpr int DP_STAGES = 5;
 constexpr int DP_STAGE_BYTES = 32768;  // A 128 x 128 bytes, B up to 128 x 128 bytes
 constexpr int DP_EPI_WARPS = 16;
+constexpr int DP_THREADS = 128 + 32 * DP_EPI_WARPS;
 
 struct DensePairSmem {
     uint8_t stage[DP_STAGES][DP_STAGE_BYTES];
@@ -48,7 +46,7 @@ struct DensePairParams {
     int T, F, bn;                    // bn: accumulator columns of a tile (gated: bn / 2 of each)
     int t_tiles, f_tiles, groups, splits;
     int kb_seg, kb_total;
-    int a_mn, b_mn, act, half, bias_fp32;
+    int a_mn, b_mn, act, bias_fp32;
     int tma_out, tma_res, save_f32;
     uint32_t idesc;
 };
@@ -111,7 +109,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 
 // ---- epilogue -------------------------------------------------------------------------------------------------------
 // v[i]: 16 columns (from `col`, a multiple of 16) of row `row` of a block of saved pre-activations; NaN and infinities keep their kind
-__device__ __forceinline__ void save_run_f16(uint8_t *values, uint8_t *exps, size_t block, int col, int row, const float (&v)[16]) {
+__device__ __forceinline__ void save_run_f16(uint8_t *values, uint8_t *exps, size_t block, int col, int row, const float *v) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
@@ -129,31 +127,26 @@ __device__ __forceinline__ void save_run_f16(uint8_t *values, uint8_t *exps, siz
     }
     exps[block * 64 + ((col & 31) >> 4) * 32 + row] = (uint8_t)(signed char)e;
 }
-__device__ __forceinline__ void save_run_f32(float *values, size_t block, int col, int row, const float (&v)[16]) {
+__device__ __forceinline__ void save_run_f32(float *values, size_t block, int col, int row, const float *v) {
     float4 *dst = reinterpret_cast<float4 *>(values + block * 1024) + ((col & 31) >> 2) * 32 + row;
 #pragma unroll
     for (int q = 0; q < 4; ++q) dst[q * 32] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
 }
-__device__ __forceinline__ void add_bias_run(float (&v)[16], const float *bias) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float4 b = reinterpret_cast<const float4 *>(bias)[i];
-        f2_unpack(f2_add(f2_pack(v[4 * i], v[4 * i + 1]), f2_pack(b.x, b.y)), v[4 * i], v[4 * i + 1]);
-        f2_unpack(f2_add(f2_pack(v[4 * i + 2], v[4 * i + 3]), f2_pack(b.z, b.w)), v[4 * i + 2], v[4 * i + 3]);
-    }
-}
-
-// The tiles of a pair in turn: item = pair + n pairs in the order (f fastest, t, group, split).  Stepping adds the digits of `pairs` with carries: a
-// division per tile would cost the one thread that issues the products several hundred cycles between tiles.
+// The tiles of a pair in turn: every pairs-th in the order (f fastest, t, group, split), so that the pairs of a moment share rows of A and columns of
+// B in L2 (a run of neighbours per pair instead: 16384 x 4096 x 4096 takes 449 us for 341, a short reduction the same).  Stepping adds the
+// digits of `pairs` with carries: a division per tile would cost the thread that issues the products several hundred cycles between tiles.
 struct DensePairTiles {
-    int f, t, gs;             // digits of the current item (gs = split * groups + group)
+    int f, t, gs, left;       // digits of the current item (gs = split * groups + group); items left, this one included
     int step_f, step_t, step_gs;
-    __device__ __forceinline__ DensePairTiles(const DensePairParams &p, int item, int pairs) {
-        f = item % p.f_tiles, t = item / p.f_tiles, gs = t / p.t_tiles, t %= p.t_tiles;
+    __device__ __forceinline__ DensePairTiles(const DensePairParams &p, int pair, int pairs) {
+        const int items = p.f_tiles * p.t_tiles * p.groups * p.splits, rest = items % pairs;
+        left = items / pairs + (pair < rest ? 1 : 0);
+        f = pair % p.f_tiles, t = pair / p.f_tiles, gs = t / p.t_tiles, t %= p.t_tiles;
         step_f = pairs % p.f_tiles, step_t = pairs / p.f_tiles, step_gs = step_t / p.t_tiles, step_t %= p.t_tiles;
     }
-    __device__ __forceinline__ bool valid(const DensePairParams &p) const { return gs < p.groups * p.splits; }
+    __device__ __forceinline__ bool valid() const { return left > 0; }
     __device__ __forceinline__ void next(const DensePairParams &p) {
+        --left;
         f += step_f, t += step_t, gs += step_gs;
         if (f >= p.f_tiles) f -= p.f_tiles, ++t;
         if (t >= p.t_tiles) t -= p.t_tiles, ++gs;
@@ -170,21 +163,10 @@ struct DensePairTiles {
     }
 };
 
-// The 16 columns from `c` of a 32-column panel: bias, saved pre-activations, activation, product, residual, rounding, into the panel.
-template <int MODE, int ACT>
-__device__ __forceinline__ void dense_pair_run(const DensePairParams &p, const uint32_t *raw, const uint32_t *raw2, const float *bias, const float *bias2,
-                                               bool has_bias, bool has_res, uint8_t *panel, int c, int col, size_t block) {
+// 16 columns (from `c` of a 32-column panel): saved pre-activations, activation, product, residual, rounding, into the panel.
+template <int MODE, int ACT, int HALF>
+__device__ __forceinline__ void dense_pair_run(const DensePairParams &p, float *v, float *u, bool has_res, uint8_t *panel, int c, int col, size_t block) {
     const int lane = threadIdx.x & 31;
-    float v[16], u[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        v[i] = __uint_as_float(raw[i]);
-        if (MODE == DP_GATED) u[i] = __uint_as_float(raw2[i]);
-    }
-    if (has_bias) {
-        add_bias_run(v, bias + c);
-        if (MODE == DP_GATED) add_bias_run(u, bias2 + c);
-    }
     if (p.save0) {
         if (p.save_f32) {
             save_run_f32(reinterpret_cast<float *>(p.save0), block, col, lane, v);
@@ -198,7 +180,7 @@ __device__ __forceinline__ void dense_pair_run(const DensePairParams &p, const u
     for (int i = 0; i < 16; i += 2) act_pair<ACT>(v[i], v[i + 1]);
     if (MODE == DP_GATED) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] *= u[i];
+        for (int i = 0; i < 16; i += 2) f2_unpack(f2_mul(f2_pack(v[i], v[i + 1]), f2_pack(u[i], u[i + 1])), v[i], v[i + 1]);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -209,22 +191,25 @@ __device__ __forceinline__ void dense_pair_run(const DensePairParams &p, const u
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float lo, hi;
-                unpack_bits16(w[i], p.half, lo, hi);
+                unpack_bits16(w[i], HALF, lo, hi);
                 v[h * 8 + 2 * i] += lo, v[h * 8 + 2 * i + 1] += hi;
             }
         }
-        *at = make_uint4(pack_bits16(v[h * 8], v[h * 8 + 1], p.half), pack_bits16(v[h * 8 + 2], v[h * 8 + 3], p.half),
-                         pack_bits16(v[h * 8 + 4], v[h * 8 + 5], p.half), pack_bits16(v[h * 8 + 6], v[h * 8 + 7], p.half));
+        *at = make_uint4(pack_bits16(v[h * 8], v[h * 8 + 1], HALF), pack_bits16(v[h * 8 + 2], v[h * 8 + 3], HALF),
+                         pack_bits16(v[h * 8 + 4], v[h * 8 + 5], HALF), pack_bits16(v[h * 8 + 6], v[h * 8 + 7], HALF));
     }
 }
 
-// Epilogue of one warp: 32 rows x a quarter of the tile's columns, in panels of 32 columns that alternate between two buffers: while one is
+// Epilogue of one warp: 32 rows x half of the tile's columns, in panels of 32 columns that alternate between two buffers: while one is
 // computed the other leaves by its TMA store, and the residual of the next panel is on its way into it as soon as that store has read it.
-template <int MODE, int ACT>
+// The accumulators of the next step are on their way from tensor memory while a step (32 columns, or 16 of each of two) is computed: beside
+// running products a tcgen05.ld takes most of a thousand cycles.
+template <int MODE, int ACT, int HALF>
 __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, DensePairSmem &sm, const CUtensorMap *my, const CUtensorMap *mr,
                                                     uint32_t tmem, uint32_t rank, DensePairTiles t) {
+    constexpr int STEP = MODE == DP_GATED ? 16 : 32, GROUPS = DP_EPI_WARPS / 4;
     const int ew = (threadIdx.x >> 5) - 4, lane = threadIdx.x & 31, q = ew & 3, g = ew >> 2;
-    const int f_width = MODE == DP_GATED ? p.bn / 2 : p.bn, panels = f_width >> 7;  // panels of this warp per tile: 2 or 1
+    const int f_width = MODE == DP_GATED ? p.bn / 2 : p.bn, panels = f_width / (32 * GROUPS);  // panels of this warp per tile: 4 or 2
     const int col_blocks = (p.F + 31) >> 5;
     const uint32_t acc_free0 = map_to_rank(smem_u32(&sm.acc_free[0]), 0), acc_free1 = map_to_rank(smem_u32(&sm.acc_free[1]), 0);
     const bool has_res = MODE == DP_LINEAR && p.residual != nullptr, res_tma = has_res && p.tma_res;
@@ -237,100 +222,122 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
             tma_load_2d(sm.panel[ew][b], mr, col_of(x, i), row_of(x), &sm.res_full[ew][b]);
         }
     };
-    float b0[2], b1[2];  // this lane's biases (column lane of each panel), fetched a tile ahead
+    // this lane's biases (column lane of each panel) as they are in memory, fetched a tile ahead and converted when used
+    uint32_t b0[4] = {0, 0, 0, 0}, b1[2] = {0, 0};
+    auto raw_bias = [&](const void *b, int c) -> uint32_t {
+        if (!b || c >= p.F) return 0;
+        return p.bias_fp32 ? reinterpret_cast<const uint32_t *>(b)[c] : reinterpret_cast<const unsigned short *>(b)[c];
+    };
+    auto to_bias = [&](uint32_t r) { return p.bias_fp32 ? __uint_as_float(r) : from_bits16((unsigned short)r, HALF); };
     auto fetch_biases = [&](const DensePairTiles &x) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int c = col_of(x, i) + lane;
-            const bool in = i < panels && c < p.F;
-            b0[i] = in && p.bias0 ? load_bias(p.bias0, c, p.bias_fp32, p.half) : 0.f;
-            if (MODE == DP_GATED) b1[i] = in && p.bias1 ? load_bias(p.bias1, c, p.bias_fp32, p.half) : 0.f;
-        }
+        for (int i = 0; i < 4; ++i)
+            if (i < panels) {
+                b0[i] = raw_bias(p.bias0, col_of(x, i) + lane);
+                if (MODE == DP_GATED && i < 2) b1[i] = raw_bias(p.bias1, col_of(x, i) + lane);
+            }
     };
     if (has_bias) fetch_biases(t);
     if (res_tma && lane == 0) fetch_residual(t, 0, 0);
     uint32_t res_phase = 0;  // bit b: phase of res_full[b]
     int used = 0;            // panels so far
-    for (int n = 0; t.valid(p); ++n) {
+    for (int n = 0; t.valid(); ++n) {
         const int row0 = row_of(t), a = n & 1;
         DensePairTiles next = t;
         next.next(p);
         if (!mbar_wait_abortable(&sm.acc_full[a], (n >> 1) & 1, &sm.abort_flag)) break;
         tc_fence_after();
+        const uint32_t acc = tmem + a * 256 + ((uint32_t)(q * 32) << 16) + g * panels * 32;
+        uint32_t raw[STEP], raw2[MODE == DP_GATED ? STEP : 1];
+        auto fetch_acc = [&](int c) {
+            if constexpr (MODE == DP_GATED) {
+                tmem_ld16(acc + c, raw);
+                tmem_ld16(acc + f_width + c, raw2);
+            } else {
+                tmem_ld32(acc + c, raw);
+            }
+        };
         // The four warps of a column group write the same biases to the same place.  Nobody still reads this buffer: the accumulator of tile n
         // became full only after every warp had released tile n - 2.
-        float *bias = &sm.bias[a][g * panels * 32], *bias2 = &sm.bias[a][128 + g * 32];
+        float *bias = &sm.bias[a][g * panels * 32], *bias2 = &sm.bias[a][128 + g * panels * 32];
         if (has_bias) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < 4; ++i)
                 if (i < panels) {
-                    bias[i * 32 + lane] = b0[i];
-                    if (MODE == DP_GATED) bias2[lane] = b1[0];
+                    bias[i * 32 + lane] = to_bias(b0[i]);
+                    if (MODE == DP_GATED && i < 2) bias2[i * 32 + lane] = to_bias(b1[i]);
                 }
-            if (next.valid(p)) fetch_biases(next);
+            if (next.valid()) fetch_biases(next);
             __syncwarp();
         }
-        const uint32_t acc = tmem + a * 256 + ((uint32_t)(q * 32) << 16) + g * panels * 32;
 #pragma unroll 1
-        for (int i = 0; i < panels; ++i, ++used) {
-            const int col = col_of(t, i), b = used & 1;
-            const bool live = row0 < p.T && col < p.F, last = i + 1 == panels;  // (warp-uniform)
+        for (int c = 0; c < panels * 32; c += STEP) {
+            const int i = c >> 5, col = col_of(t, i), b = used & 1;
+            const bool live = row0 < p.T && col < p.F;  // (warp-uniform)
+            const bool first = (c & 31) == 0, last = ((c + STEP) & 31) == 0;
             uint8_t *panel = sm.panel[ew][b];
-            if (MODE != DP_PARTIAL && !res_tma) {
-                if (lane == 0) bulk_wait_read<1>();  // the store before the last one has read this buffer
-                __syncwarp();
-            }
-            if (has_res && !p.tma_res && live) {  // any alignment: a row at a time, a column per lane
-#pragma unroll 4
-                for (int r = 0; r < 32; ++r) {
-                    const unsigned short v = row0 + r < p.T && col + lane < p.F ? p.residual[(long long)(row0 + r) * p.ld_res + col + lane] : (unsigned short)0;
-                    *reinterpret_cast<unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2) = v;
+            if (MODE != DP_PARTIAL && first) {
+                if (res_tma) {
+                    if (live) {
+                        mbar_wait_abortable(&sm.res_full[ew][b], (res_phase >> b) & 1, &sm.abort_flag);
+                        res_phase ^= 1u << b;
+                    }
+                } else {
+                    if (lane == 0) bulk_wait_read<1>();  // the store before the last one has read this buffer
+                    __syncwarp();
                 }
-                __syncwarp();
+                if (has_res && !p.tma_res && live) {  // any alignment: a row at a time, a column per lane
+#pragma unroll 4
+                    for (int r = 0; r < 32; ++r) {
+                        const unsigned short v =
+                            row0 + r < p.T && col + lane < p.F ? p.residual[(long long)(row0 + r) * p.ld_res + col + lane] : (unsigned short)0;
+                        *reinterpret_cast<unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2) = v;
+                    }
+                    __syncwarp();
+                }
             }
-            const size_t block = saved_block(row0, col, col_blocks);
-            auto release = [&]() {  // the accumulator has been read: the products may have it back
+            float v[STEP], u[MODE == DP_GATED ? STEP : 1];
+            fetch_acc(c);
+            tmem_wait_ld();
+            if (has_bias) {
+#pragma unroll
+                for (int k = 0; k < STEP; k += 4) {
+                    const float4 w = *reinterpret_cast<const float4 *>(bias + c + k);
+                    f2_unpack(f2_add(f2_pack(__uint_as_float(raw[k]), __uint_as_float(raw[k + 1])), f2_pack(w.x, w.y)), v[k], v[k + 1]);
+                    f2_unpack(f2_add(f2_pack(__uint_as_float(raw[k + 2]), __uint_as_float(raw[k + 3])), f2_pack(w.z, w.w)), v[k + 2], v[k + 3]);
+                    if constexpr (MODE == DP_GATED) {
+                        const float4 x = *reinterpret_cast<const float4 *>(bias2 + c + k);
+                        f2_unpack(f2_add(f2_pack(__uint_as_float(raw2[k]), __uint_as_float(raw2[k + 1])), f2_pack(x.x, x.y)), u[k], u[k + 1]);
+                        f2_unpack(f2_add(f2_pack(__uint_as_float(raw2[k + 2]), __uint_as_float(raw2[k + 3])), f2_pack(x.z, x.w)), u[k + 2], u[k + 3]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < STEP; ++k) {
+                    v[k] = __uint_as_float(raw[k]);
+                    if constexpr (MODE == DP_GATED) u[k] = __uint_as_float(raw2[k]);
+                }
+            }
+            if (c + STEP == panels * 32) {  // the accumulator has been read: the products may have it back
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(a ? acc_free1 : acc_free0);
-            };
-            if (MODE == DP_GATED) {
-#pragma unroll 1
-                for (int c = 0; c < 32; c += 16) {
-                    uint32_t raw[16], raw2[16];
-                    tmem_ld16(acc + c, raw);
-                    tmem_ld16(acc + f_width + c, raw2);
-                    tmem_wait_ld();
-                    if (c == 16) release();
-                    if (live) dense_pair_run<MODE, ACT>(p, raw, raw2, bias, bias2, has_bias, false, panel, c, col + c, block);
-                }
-            } else {
-                uint32_t raw[32];
-                tmem_ld32(acc + i * 32, raw);
-                tmem_wait_ld();
-                if (last) release();
-                if (live && res_tma) {
-                    mbar_wait_abortable(&sm.res_full[ew][b], (res_phase >> b) & 1, &sm.abort_flag);
-                    res_phase ^= 1u << b;
-                }
-                if (live) {
-                    if (MODE == DP_PARTIAL) {
-                        float *part = p.part + (size_t)t.gs * (saved_bytes_f32(p.T, p.F) / 4);
-#pragma unroll
-                        for (int c = 0; c < 32; c += 16) {
-                            float v[16];
-#pragma unroll
-                            for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(raw[c + k]);
-                            save_run_f32(part, block, c, lane, v);
-                        }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 32; c += 16)
-                            dense_pair_run<MODE, ACT>(p, raw + c, nullptr, bias + i * 32, nullptr, has_bias, has_res, panel, c, col + c, block);
-                    }
-                }
             }
-            if (MODE == DP_PARTIAL) continue;
+            const size_t block = saved_block(row0, col, col_blocks);
+            if (MODE == DP_PARTIAL) {
+                if (live) {
+                    float *part = p.part + (size_t)t.gs * (saved_bytes_f32(p.T, p.F) / 4);
+#pragma unroll
+                    for (int k = 0; k < STEP; k += 16) save_run_f32(part, block, k, lane, v + k);
+                }
+                continue;
+            }
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < STEP; k += 16) dense_pair_run<MODE, ACT, HALF>(p, v + k, u, has_res, panel, (c & 31) + k, col + (c & 31) + k, block);
+            }
+            if (!last) continue;
+            ++used;
             if (p.tma_out) {
                 fence_proxy_async();
                 __syncwarp();
@@ -343,14 +350,15 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
 #pragma unroll 4
                 for (int r = 0; r < 32; ++r)
                     if (row0 + r < p.T && col + lane < p.F)
-                        p.out0[(long long)(row0 + r) * p.ld_out + col + lane] = *reinterpret_cast<const unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2);
+                        p.out0[(long long)(row0 + r) * p.ld_out + col + lane] =
+                            *reinterpret_cast<const unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2);
                 __syncwarp();
             }
             if (res_tma && lane == 0) {  // the next panel's residual into the other buffer, once the store before this one has read it
                 bulk_wait_read<1>();
                 fence_proxy_async();
-                if (!last) fetch_residual(t, i + 1, b ^ 1);
-                else if (next.valid(p)) fetch_residual(next, 0, b ^ 1);
+                if (i + 1 < panels) fetch_residual(t, i + 1, b ^ 1);
+                else if (next.valid()) fetch_residual(next, 0, b ^ 1);
             }
             __syncwarp();
         }
@@ -360,7 +368,7 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
     __syncwarp();
 }
 
-template <int MODE>
+template <int MODE, int HALF>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
     dense_pair_kernel(const __grid_constant__ CUtensorMap ma0, const __grid_constant__ CUtensorMap ma1, const __grid_constant__ CUtensorMap mb0,
                       const __grid_constant__ CUtensorMap mb1, const __grid_constant__ CUtensorMap my, const __grid_constant__ CUtensorMap mr,
@@ -408,7 +416,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
         uint32_t phase = 0;
         bool ok = true;
         const uint32_t bytes = 2 * (16384 + (uint32_t)b_rows * 128), full0 = map_to_rank(smem_u32(&sm.full[0]), 0);
-        for (; t.valid(p) && ok; t.next(p)) {
+        for (; t.valid() && ok; t.next(p)) {
             const int ta = t.t * 256 + (int)rank * 128, fb = t.f * f_width + (MODE == DP_GATED ? 0 : (int)rank * b_rows), group = t.group(p);
             int k0, k1;
             t.range(p, k0, k1);
@@ -450,7 +458,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
             int slot = 0;
             uint32_t phase = 0;
             bool ok = true;
-            for (int n = 0; t.valid(p) && ok; t.next(p), ++n) {
+            for (int n = 0; t.valid() && ok; t.next(p), ++n) {
                 const int acc = n & 1;
                 int k0, k1;
                 t.range(p, k0, k1);
@@ -477,14 +485,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
         }
     } else if (warp >= 4) {
         if (MODE == DP_PARTIAL) {
-            dense_pair_epilogue<MODE, ACT_NONE>(p, sm, &my, &mr, tmem, rank, t);
+            dense_pair_epilogue<MODE, ACT_NONE, HALF>(p, sm, &my, &mr, tmem, rank, t);
         } else {
             switch (p.act) {
-                case ACT_GELU: dense_pair_epilogue<MODE, ACT_GELU>(p, sm, &my, &mr, tmem, rank, t); break;
-                case ACT_SILU: dense_pair_epilogue<MODE, ACT_SILU>(p, sm, &my, &mr, tmem, rank, t); break;
-                case ACT_RELU: dense_pair_epilogue<MODE, ACT_RELU>(p, sm, &my, &mr, tmem, rank, t); break;
-                case ACT_SIGMOID: dense_pair_epilogue<MODE, ACT_SIGMOID>(p, sm, &my, &mr, tmem, rank, t); break;
-                default: dense_pair_epilogue<MODE, ACT_NONE>(p, sm, &my, &mr, tmem, rank, t);
+                case ACT_GELU: dense_pair_epilogue<MODE, ACT_GELU, HALF>(p, sm, &my, &mr, tmem, rank, t); break;
+                case ACT_SILU: dense_pair_epilogue<MODE, ACT_SILU, HALF>(p, sm, &my, &mr, tmem, rank, t); break;
+                case ACT_RELU: dense_pair_epilogue<MODE, ACT_RELU, HALF>(p, sm, &my, &mr, tmem, rank, t); break;
+                case ACT_SIGMOID: dense_pair_epilogue<MODE, ACT_SIGMOID, HALF>(p, sm, &my, &mr, tmem, rank, t); break;
+                default: dense_pair_epilogue<MODE, ACT_NONE, HALF>(p, sm, &my, &mr, tmem, rank, t);
             }
         }
     }
