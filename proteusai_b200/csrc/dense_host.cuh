@@ -107,13 +107,13 @@ static DenseChoice dense_choose(const DenseProduct &d, int sms, bool may_split) 
     return b.cost < a.cost ? b : a;
 }
 
-template <bool DUAL>
+template <bool DUAL, int HALF>
 static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams &p, long long ctas, int smem, cudaStream_t st) {
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(dense_tile_kernel<DUAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        cudaError_t e = cudaFuncSetAttribute(dense_tile_kernel<DUAL, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
@@ -128,7 +128,7 @@ static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, dense_tile_kernel<DUAL>, m[0], m[1], m[2], m[3], p);
+    return (int)cudaLaunchKernelEx(&cfg, dense_tile_kernel<DUAL, HALF>, m[0], m[1], m[2], m[3], p);
 }
 
 static uint32_t dense_idesc(int m, int n, const DenseProduct &d, int m_mn, int n_mn) {
@@ -148,7 +148,7 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
     p.splits = splits, p.tn = tn;
     p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
     p.a_mn = d.a_mn, p.b_mn = d.b_mn;
-    p.act = d.act, p.half = d.half, p.bias_fp32 = d.bias_fp32;
+    p.act = d.act, p.bias_fp32 = d.bias_fp32;
     p.idesc = dense_idesc(128, tn, d, d.a_mn, d.b_mn);
     const long long ctas = (long long)p.f_tiles * p.t_tiles * d.groups * splits;
     if (ctas > 0x7fffffffll) return (int)PAI_ERR_BAD_SHAPE;
@@ -168,7 +168,8 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
         if (i == 1 && !d.b[1].p) m[3] = m[2];
         else if (int e = d.b_mn ? make_map_16(&m[2 + i], b.p, d.T, d.R, b.ld, 64, d.half) : make_map_16(&m[2 + i], b.p, d.R, d.T, b.ld, tn, d.half)) return e;
     }
-    return d.dual ? dense_tile_launch_as<true>(m, p, ctas, smem, st) : dense_tile_launch_as<false>(m, p, ctas, smem, st);
+    if (d.half) return d.dual ? dense_tile_launch_as<true, 1>(m, p, ctas, smem, st) : dense_tile_launch_as<false, 1>(m, p, ctas, smem, st);
+    return d.dual ? dense_tile_launch_as<true, 0>(m, p, ctas, smem, st) : dense_tile_launch_as<false, 0>(m, p, ctas, smem, st);
 }
 
 // map of an operand as MMA rows (`rows` of them, `box` per load): reduction-contiguous or not
@@ -316,6 +317,29 @@ static size_t dense_bwd_workspace(long long M, int N, int K, int mats, int sms) 
     return mats * (dense_d_bytes(M, N) + dense_part_bytes(M, N)) + dense_split_bytes(M, N, K, mats, sms);
 }
 
+template <bool DUAL, int ACT>
+static void dense_bwd_elem_as(const DenseBwdElemParams &p, int half, bool f32, dim3 grid, cudaStream_t st) {
+    if (half) dense_bwd_elem_kernel<DUAL, ACT, 1, true><<<grid, 256, 0, st>>>(p);
+    else if (f32) dense_bwd_elem_kernel<DUAL, ACT, 0, true><<<grid, 256, 0, st>>>(p);
+    else dense_bwd_elem_kernel<DUAL, ACT, 0, false><<<grid, 256, 0, st>>>(p);
+}
+template <bool DUAL>
+static void dense_bwd_elem_act(const DenseBwdElemParams &p, int act, int half, bool f32, dim3 grid, cudaStream_t st) {
+    switch (act) {
+        case ACT_GELU: return dense_bwd_elem_as<DUAL, ACT_GELU>(p, half, f32, grid, st);
+        case ACT_SILU: return dense_bwd_elem_as<DUAL, ACT_SILU>(p, half, f32, grid, st);
+        case ACT_RELU: return dense_bwd_elem_as<DUAL, ACT_RELU>(p, half, f32, grid, st);
+        case ACT_SIGMOID: return dense_bwd_elem_as<DUAL, ACT_SIGMOID>(p, half, f32, grid, st);
+        default: return dense_bwd_elem_as<DUAL, ACT_NONE>(p, half, f32, grid, st);
+    }
+}
+static int dense_bwd_elem_launch(const DenseBwdElemParams &p, bool gated, int act, int half, bool f32, unsigned strips, cudaStream_t st) {
+    const dim3 grid((p.N + 255) / 256, strips);
+    if (gated) dense_bwd_elem_act<true>(p, act, half, f32, grid, st);
+    else dense_bwd_elem_act<false>(p, act, half, f32, grid, st);
+    return (int)cudaPeekAtLastError();
+}
+
 static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const DenseOperand (&w)[2], const void *saved, void *dx, long long lddx,
                           void *const (&dw)[2], void *const (&db)[2], int bias_fp32, void *workspace, long long M, int N, int K, int act, int half,
                           int sms, cudaStream_t st) {
@@ -329,11 +353,11 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
     DenseBwdElemParams p = {};
     p.dy = (const unsigned short *)dy.p, p.ld_dy = dy.ld;
     p.vec_dy = ((uintptr_t)dy.p & 15) == 0 && (dy.ld & 7) == 0;
-    p.M = M, p.N = N, p.act = act, p.half = half, p.strip = dense_strip_rows(M, N);
+    p.M = M, p.N = N, p.strip = dense_strip_rows(M, N);
+    const bool f32 = dense_saves_f32(M, N, K, gated, half, sms);
     if (elementwise) {
         p.save0 = (const uint8_t *)saved;
         p.save1 = gated ? (const uint8_t *)saved + dense_saved_matrix(M, N, K, gated, half, sms) : nullptr;
-        p.save_f32 = dense_saves_f32(M, N, K, gated, half, sms);
         p.save_exps = saved_blocks(M, N) * 2048;
         if (products) {
             p.ld_d = dense_ld16(N);
@@ -347,10 +371,7 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
         p.part1 = gated ? p.part0 + dense_part_bytes(M, N) / 4 : nullptr;
     }
     if ((elementwise && products) || p.part0) {
-        const dim3 grid((N + 255) / 256, (unsigned)strips);
-        if (gated) dense_bwd_elem_kernel<true><<<grid, 256, 0, st>>>(p);
-        else dense_bwd_elem_kernel<false><<<grid, 256, 0, st>>>(p);
-        if (int e = (int)cudaPeekAtLastError()) return e;
+        if (int e = dense_bwd_elem_launch(p, gated, act, half, f32, (unsigned)strips, st)) return e;
     }
     if (p.part0) {
         // (one of two bias gradients alone: its own sums go into the grid's first row)

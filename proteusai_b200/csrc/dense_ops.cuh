@@ -73,29 +73,24 @@ __device__ __forceinline__ void act_pair(float &a, float &b) {
 }
 
 // act(z) and act'(z)
-__device__ __forceinline__ void act_and_slope(int act, float z, float &a, float &d) {
-    switch (act) {
-        case ACT_GELU: {
-            const float n = fmaxf(-fabsf(z), -30.f), e = normal_tail(n), phi = z < 0.f ? e : 1.f - e;
-            a = fmaf(n, e, max_nan(z, 0.f));
-            d = fmaf(z * 0.3989422804014327f, ex2_approx(-0.7213475204444817f * z * z), phi);
-            break;
-        }
-        case ACT_SILU: {
-            const float s = sigmoid_f(z);
-            a = z * s;
-            d = s * fmaf(z, 1.f - s, 1.f);
-            break;
-        }
-        case ACT_RELU:
-            a = max_nan(z, 0.f);
-            d = z > 0.f ? 1.f : 0.f;
-            break;
-        case ACT_SIGMOID:
-            a = sigmoid_f(z);
-            d = a * (1.f - a);
-            break;
-        default: a = z, d = 1.f;
+template <int ACT>
+__device__ __forceinline__ void act_and_slope(float z, float &a, float &d) {
+    if (ACT == ACT_GELU) {
+        const float n = fmaxf(-fabsf(z), -30.f), e = normal_tail(n), phi = z < 0.f ? e : 1.f - e;
+        a = fmaf(n, e, max_nan(z, 0.f));
+        d = fmaf(z * 0.3989422804014327f, ex2_approx(-0.7213475204444817f * z * z), phi);
+    } else if (ACT == ACT_SILU) {
+        const float s = sigmoid_f(z);
+        a = z * s;
+        d = s * fmaf(z, 1.f - s, 1.f);
+    } else if (ACT == ACT_RELU) {
+        a = max_nan(z, 0.f);
+        d = z > 0.f ? 1.f : 0.f;
+    } else if (ACT == ACT_SIGMOID) {
+        a = sigmoid_f(z);
+        d = a * (1.f - a);
+    } else {
+        a = z, d = 1.f;
     }
 }
 
@@ -137,46 +132,58 @@ __device__ __forceinline__ size_t saved_block(long long row, int col, int col_bl
 __device__ __forceinline__ size_t saved_index_f32(long long row, int col, int col_blocks) {
     return (saved_block(row, col, col_blocks) * 8 + ((col & 31) >> 2)) * 128 + (size_t)(row & 31) * 4 + (col & 3);
 }
-// eight columns (col a multiple of 8) of a row
-__device__ __forceinline__ void saved_load8(const uint8_t *save, int f32, size_t exps, long long row, int col, int col_blocks, float (&z)[8]) {
-    if (f32) {
-        const float *src = reinterpret_cast<const float *>(save) + saved_index_f32(row, col, col_blocks);
-        const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 128);
-        z[0] = a.x, z[1] = a.y, z[2] = a.z, z[3] = a.w, z[4] = b.x, z[5] = b.y, z[6] = b.z, z[7] = b.w;
-    } else {
+// eight columns (col a multiple of 8) of a row: the loads, and the values from what they brought
+template <bool F32>
+struct Saved8 {
+    uint4 v[F32 ? 2 : 1];
+    int e;
+    __device__ __forceinline__ void load(const uint8_t *save, size_t exps, long long row, int col, int col_blocks) {
         const size_t block = saved_block(row, col, col_blocks);
-        const uint4 v = *reinterpret_cast<const uint4 *>(save + block * 2048 + ((col & 31) >> 3) * 512 + (row & 31) * 16);
-        const int e = reinterpret_cast<const signed char *>(save)[exps + block * 64 + ((col & 31) >> 4) * 32 + (row & 31)];
-        const float s = __uint_as_float((uint32_t)(127 + e) << 23);
-        unpack_bits16(v.x, 1, z[0], z[1]);
-        unpack_bits16(v.y, 1, z[2], z[3]);
-        unpack_bits16(v.z, 1, z[4], z[5]);
-        unpack_bits16(v.w, 1, z[6], z[7]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] *= s;
+        if (F32) {
+            const uint4 *src = reinterpret_cast<const uint4 *>(save + block * 4096) + ((col & 31) >> 2) * 32 + (row & 31);
+            v[0] = src[0], v[F32 ? 1 : 0] = src[32];
+        } else {
+            v[0] = reinterpret_cast<const uint4 *>(save + block * 2048)[((col & 31) >> 3) * 32 + (row & 31)];
+            e = reinterpret_cast<const signed char *>(save)[exps + block * 64 + ((col & 31) >> 4) * 32 + (row & 31)];
+        }
     }
-}
+    __device__ __forceinline__ void get(float (&z)[8]) const {
+        const uint32_t w[8] = {v[0].x, v[0].y, v[0].z, v[0].w, v[F32 ? 1 : 0].x, v[F32 ? 1 : 0].y, v[F32 ? 1 : 0].z, v[F32 ? 1 : 0].w};
+        if (F32) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) z[i] = __uint_as_float(w[i]);
+        } else {
+            const float s = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                unpack_bits16(w[i], 1, z[2 * i], z[2 * i + 1]);
+                z[2 * i] *= s, z[2 * i + 1] *= s;
+            }
+        }
+    }
+};
 
 // ---- elementwise half of the backward pass ------------------------------------------------------------------------
 // One warp covers 8 rows x 32 columns a step (4 lanes x 8 columns per row), a CTA 8 rows x 256 columns; it walks down a strip of
-// `strip` rows and keeps the column sums of what it writes in registers (the bias gradients), joined over the eight row lanes by
-// shuffles and written as one partial row per strip; dense_colsum_kernel adds the strips in order, so the sums are reproducible.
-// HBM-bound: linear reads dy (2 B) and z (4 B) and writes dz (2 B) per element.
+// `strip` rows, two steps' loads in flight, and keeps the column sums of what it writes in registers (the bias gradients), joined over the
+// eight row lanes by shuffles and written as one partial row per strip; dense_colsum_kernel adds the strips in order, so the sums are
+// reproducible.  HBM-bound: gated in bf16 reads dh, g, u and writes dg, du, 10 bytes per element.
 struct DenseBwdElemParams {
     const unsigned short *dy;
     long long ld_dy;
     const uint8_t *save0, *save1;   // z, or g and u
     size_t save_exps;               // fp16 form: offset of the exponents
-    int save_f32;
-    unsigned short *d0, *d1;        // dz, or dg and du; NULL: not wanted (d0: sums of dy alone)
+    unsigned short *d0, *d1;        // dz, or dg and du; NULL: not wanted
     long long ld_d;
     float *part0, *part1;           // [strips, N] column sums, or NULL
     long long M;
-    int N, act, half, strip, vec_dy;
+    int N, strip, vec_dy;
 };
 
-template <bool DUAL>
+template <bool DUAL, int ACT, int HALF, bool F32>
 __global__ void __launch_bounds__(256) dense_bwd_elem_kernel(const __grid_constant__ DenseBwdElemParams p) {
+    constexpr bool PLAIN = !DUAL && ACT == ACT_NONE;  // sums of dy alone
+    constexpr int U = 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c0 = blockIdx.x * 256 + warp * 32 + (lane & 3) * 8;
     const long long r_begin = (long long)blockIdx.y * p.strip;
@@ -187,58 +194,61 @@ __global__ void __launch_bounds__(256) dense_bwd_elem_kernel(const __grid_consta
     for (int i = 0; i < 8; ++i) s0[i] = s1[i] = 0.f;
     const int nc = p.N - c0;  // columns of this thread that exist (may be <= 0 or > 8)
     if (nc > 0) {
-        for (long long r = r_begin + (lane >> 2); r < r_end; r += 8) {
-            float dy[8];
-            const unsigned short *src = p.dy + r * p.ld_dy + c0;
-            if (p.vec_dy && nc >= 8) {
-                const uint4 v = *reinterpret_cast<const uint4 *>(src);
-                unpack_bits16(v.x, p.half, dy[0], dy[1]);
-                unpack_bits16(v.y, p.half, dy[2], dy[3]);
-                unpack_bits16(v.z, p.half, dy[4], dy[5]);
-                unpack_bits16(v.w, p.half, dy[6], dy[7]);
-            } else {
+        const bool vec = p.vec_dy && nc >= 8;
+        for (long long r0 = r_begin + (lane >> 2); r0 < r_end; r0 += 8 * U) {
+            uint32_t w[U][4];
+            Saved8<F32> z[U], u[U];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) dy[i] = i < nc ? from_bits16(src[i], p.half) : 0.f;
-            }
-            float o0[8], o1[8];
-            if (p.save0) {
-                float z[8];
-                saved_load8(p.save0, p.save_f32, p.save_exps, r, c0, col_blocks, z);
-                if (DUAL) {
-                    float u[8];
-                    saved_load8(p.save1, p.save_f32, p.save_exps, r, c0, col_blocks, u);
+            for (int k = 0; k < U; ++k) {
+                const long long r = r0 + 8 * k;
+                if (r < r_end) {
+                    const unsigned short *src = p.dy + r * p.ld_dy + c0;
+                    if (vec) {
+                        const uint4 v = *reinterpret_cast<const uint4 *>(src);
+                        w[k][0] = v.x, w[k][1] = v.y, w[k][2] = v.z, w[k][3] = v.w;
+                    } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        float a, d;
-                        act_and_slope(p.act, z[i], a, d);
-                        o0[i] = dy[i] * u[i] * d;
-                        o1[i] = dy[i] * a;
+                        for (int i = 0; i < 4; ++i)
+                            w[k][i] = (2 * i < nc ? (uint32_t)src[2 * i] : 0u) | (2 * i + 1 < nc ? (uint32_t)src[2 * i + 1] << 16 : 0u);
                     }
-                } else {
+                    if (!PLAIN) z[k].load(p.save0, p.save_exps, r, c0, col_blocks);
+                    if (DUAL) u[k].load(p.save1, p.save_exps, r, c0, col_blocks);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < U; ++k) {
+                const long long r = r0 + 8 * k;
+                if (r < r_end) {
+                    float o0[8], o1[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) unpack_bits16(w[k][i], HALF, o0[2 * i], o0[2 * i + 1]);
+                    if (!PLAIN) {
+                        float zz[8], uu[8];
+                        z[k].get(zz);
+                        if (DUAL) u[k].get(uu);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float a, d;
+                            act_and_slope<ACT>(zz[i], a, d);
+                            if (DUAL) o1[i] = o0[i] * a, d *= uu[i];
+                            o0[i] *= d;
+                        }
+                    }
+                    // (columns past N: dy is 0 there but z is not defined; their sums are never stored)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        float a, d;
-                        act_and_slope(p.act, z[i], a, d);
-                        o0[i] = dy[i] * d;
+                        s0[i] += o0[i];
+                        if (DUAL) s1[i] += o1[i];
+                    }
+                    if (!PLAIN && p.d0) {  // rows of d0 / d1 are padded to a multiple of 8 columns: whole 16-byte words, the tail is never read
+                        *reinterpret_cast<uint4 *>(p.d0 + r * p.ld_d + c0) = make_uint4(pack_bits16(o0[0], o0[1], HALF), pack_bits16(o0[2], o0[3], HALF),
+                                                                                       pack_bits16(o0[4], o0[5], HALF), pack_bits16(o0[6], o0[7], HALF));
+                        if (DUAL)
+                            *reinterpret_cast<uint4 *>(p.d1 + r * p.ld_d + c0) =
+                                make_uint4(pack_bits16(o1[0], o1[1], HALF), pack_bits16(o1[2], o1[3], HALF), pack_bits16(o1[4], o1[5], HALF),
+                                           pack_bits16(o1[6], o1[7], HALF));
                     }
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) o0[i] = dy[i];
-            }
-            // (columns past N: dy is 0 there but z is not defined; they are never written and their sums never stored)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s0[i] += o0[i];
-                if (DUAL) s1[i] += o1[i];
-            }
-            if (p.d0) {  // rows of d0 / d1 are padded to a multiple of 8 columns: whole 16-byte words, the tail is never read
-                *reinterpret_cast<uint4 *>(p.d0 + r * p.ld_d + c0) = make_uint4(pack_bits16(o0[0], o0[1], p.half), pack_bits16(o0[2], o0[3], p.half),
-                                                                               pack_bits16(o0[4], o0[5], p.half), pack_bits16(o0[6], o0[7], p.half));
-                if (DUAL)
-                    *reinterpret_cast<uint4 *>(p.d1 + r * p.ld_d + c0) =
-                        make_uint4(pack_bits16(o1[0], o1[1], p.half), pack_bits16(o1[2], o1[3], p.half), pack_bits16(o1[4], o1[5], p.half),
-                                   pack_bits16(o1[6], o1[7], p.half));
             }
         }
     }

@@ -64,12 +64,6 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 }
 // Byte offset of the 16-byte chunk `chunk` (0..3) of row `row` inside a [rows x 64 B] tile stored with the 64-byte swizzle.
 __device__ __forceinline__ uint32_t sw64_offset(int row, int chunk) { return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); }
-// one thread of a converged warp
-__device__ __forceinline__ bool elect_one() {
-    uint32_t r;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-    return r != 0;
-}
 // load into this CTA's shared memory, completion on a barrier of either CTA of the pair (`bar`: shared::cluster address)
 __device__ __forceinline__ void tma_load_2d_pair(void *dst_smem, const CUtensorMap *map, int c0, int c1, uint32_t bar) {
     asm volatile(

@@ -36,7 +36,7 @@ struct DenseTileParams {
     int f_tiles, t_tiles, splits, tn, stages;
     int kb_seg, kb_total;           // 64-wide reduction blocks of the first operand pair, of both
     int a_mn, b_mn;                 // operands stored with the reduction as their slow axis
-    int act, half, bias_fp32;
+    int act, bias_fp32;
     uint32_t idesc;
 };
 
@@ -48,6 +48,12 @@ __device__ __forceinline__ void tma_load_2d(void *dst_smem, const CUtensorMap *m
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// one thread of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
     float v;
     asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
@@ -75,7 +81,7 @@ __device__ __forceinline__ float dense_finish(const DenseTileParams &p, float v0
     return DUAL ? v0 * v1 : v0;
 }
 
-template <bool DUAL, int ACT>
+template <bool DUAL, int ACT, int HALF>
 __device__ __forceinline__ void dense_epilogue(const DenseTileParams &p, uint32_t tmem, float *red, int f0, int t0, int group, int rank) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     unsigned short *out = reinterpret_cast<unsigned short *>(group ? p.out1 : p.out0);
@@ -83,8 +89,8 @@ __device__ __forceinline__ void dense_epilogue(const DenseTileParams &p, uint32_
     if (p.splits == 1) {
         const int q = warp & 3, f = f0 + q * 32 + lane;
         const bool live = f < p.F;
-        const float b0 = live && p.bias0 ? load_bias(p.bias0, f, p.bias_fp32, p.half) : 0.f;
-        const float b1 = DUAL && live && p.bias1 ? load_bias(p.bias1, f, p.bias_fp32, p.half) : 0.f;
+        const float b0 = live && p.bias0 ? load_bias(p.bias0, f, p.bias_fp32, HALF) : 0.f;
+        const float b1 = DUAL && live && p.bias1 ? load_bias(p.bias1, f, p.bias_fp32, HALF) : 0.f;
         for (int c = (warp >> 2) * 16; c < p.tn; c += 32) {
             if (t0 + c >= p.T) break;  // (warp-uniform)
             uint32_t v[16], u[16];
@@ -94,7 +100,7 @@ __device__ __forceinline__ void dense_epilogue(const DenseTileParams &p, uint32_
             const int nt = p.T - t0 - c;
             if (p.residual) {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) r[j] = (live && j < nt) ? from_bits16(p.residual[(long long)(t0 + c + j) * p.ld_res + f], p.half) : 0.f;
+                for (int j = 0; j < 16; ++j) r[j] = (live && j < nt) ? from_bits16(p.residual[(long long)(t0 + c + j) * p.ld_res + f], HALF) : 0.f;
             } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) r[j] = 0.f;
@@ -106,34 +112,44 @@ __device__ __forceinline__ void dense_epilogue(const DenseTileParams &p, uint32_
                     if (j < nt) {
                         const int t = t0 + c + j;
                         const float y = dense_finish<DUAL, ACT>(p, __uint_as_float(v[j]), DUAL ? __uint_as_float(u[j]) : 0.f, b0, b1, f, t, col_blocks);
-                        out[(long long)t * p.ld_out + f] = to_bits16(y + r[j], p.half);
+                        out[(long long)t * p.ld_out + f] = to_bits16(y + r[j], HALF);
                     }
             }
+            __syncwarp();
         }
         return;
     }
     // the cluster's partial tiles: rows [rank, rank + 1) tn / splits of the tile are this CTA's to finish
     const int fl = tid & 127, f = f0 + fl;
     if (f >= p.F) return;
-    const float b0 = p.bias0 ? load_bias(p.bias0, f, p.bias_fp32, p.half) : 0.f;
-    const float b1 = DUAL && p.bias1 ? load_bias(p.bias1, f, p.bias_fp32, p.half) : 0.f;
+    const float b0 = p.bias0 ? load_bias(p.bias0, f, p.bias_fp32, HALF) : 0.f;
+    const float b1 = DUAL && p.bias1 ? load_bias(p.bias1, f, p.bias_fp32, HALF) : 0.f;
     const int rows = p.tn / p.splits;
     for (int j = tid >> 7; j < rows; j += 2) {
         const int tl = rank * rows + j, t = t0 + tl;
         if (t >= p.T) break;
-        float v0 = 0.f, v1 = 0.f;
         const uint32_t at = smem_u32(red + (size_t)tl * DT_FT + fl);
-        for (int s = 0; s < p.splits; ++s) {
-            v0 += ld_cluster_f32(at, s);
-            if (DUAL) v1 += ld_cluster_f32(at + (uint32_t)p.tn * DT_FT * 4, s);
-        }
-        float y = dense_finish<DUAL, ACT>(p, v0, v1, b0, b1, f, t, col_blocks);
-        if (p.residual) y += from_bits16(p.residual[(long long)t * p.ld_res + f], p.half);
-        out[(long long)t * p.ld_out + f] = to_bits16(y, p.half);
+        float part0[8], part1[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // all ranks' values on their way at once
+            if (i < p.splits) {
+                part0[i] = ld_cluster_f32(at, i);
+                if (DUAL) part1[i] = ld_cluster_f32(at + (uint32_t)p.tn * DT_FT * 4, i);
+            }
+        const float r = p.residual ? from_bits16(p.residual[(long long)t * p.ld_res + f], HALF) : 0.f;
+        float v0 = part0[0], v1 = DUAL ? part1[0] : 0.f;
+#pragma unroll
+        for (int i = 1; i < 8; ++i)
+            if (i < p.splits) {
+                v0 += part0[i];
+                if (DUAL) v1 += part1[i];
+            }
+        const float y = dense_finish<DUAL, ACT>(p, v0, v1, b0, b1, f, t, col_blocks);
+        out[(long long)t * p.ld_out + f] = to_bits16(y + r, HALF);
     }
 }
 
-template <bool DUAL>
+template <bool DUAL, int HALF>
 __global__ void __launch_bounds__(DT_THREADS) dense_tile_kernel(const __grid_constant__ CUtensorMap ma0, const __grid_constant__ CUtensorMap ma1,
                                                                 const __grid_constant__ CUtensorMap mb0, const __grid_constant__ CUtensorMap mb1,
                                                                 const __grid_constant__ DenseTileParams p) {
@@ -167,35 +183,42 @@ __global__ void __launch_bounds__(DT_THREADS) dense_tile_kernel(const __grid_con
     tc_fence_after();
     const uint32_t tmem = tmem_base;
 
-    if (warp == 0 && lane == 0) {
+    // (the whole warp runs the loop, one elected thread issues: control flow and descriptors stay warp-uniform)
+    if (warp == 0) {
+        const bool leader = elect_one();
         int slot = 0;
         uint32_t phase = 0;
         for (int kb = k0; kb < k1; ++kb) {
             if (!mbar_wait_abortable(&bar_free[slot], phase ^ 1, &abort_flag)) break;
-            uint8_t *a = base + (size_t)slot * stage_bytes, *b = a + a_bytes;
-            mbar_expect_tx(&bar_full[slot], stage_bytes);
-            const bool second = kb >= p.kb_seg;
-            const int r = (second ? kb - p.kb_seg : kb) * DT_BK;
-            const CUtensorMap *ma = second ? &ma1 : &ma0, *mb = (second || group) ? &mb1 : &mb0;
-            if (p.a_mn) {
-                tma_load_2d(a, ma, f0, r, &bar_full[slot]);
-                tma_load_2d(a + 8192, ma, f0 + 64, r, &bar_full[slot]);
-            } else {
-                tma_load_2d(a, ma, r, f0, &bar_full[slot]);
-                if (DUAL) tma_load_2d(a + 16384, &ma1, r, f0, &bar_full[slot]);
+            if (leader) {
+                uint8_t *a = base + (size_t)slot * stage_bytes, *b = a + a_bytes;
+                mbar_expect_tx(&bar_full[slot], stage_bytes);
+                const bool second = kb >= p.kb_seg;
+                const int r = (second ? kb - p.kb_seg : kb) * DT_BK;
+                const CUtensorMap *ma = second ? &ma1 : &ma0, *mb = (second || group) ? &mb1 : &mb0;
+                if (p.a_mn) {
+                    tma_load_2d(a, ma, f0, r, &bar_full[slot]);
+                    tma_load_2d(a + 8192, ma, f0 + 64, r, &bar_full[slot]);
+                } else {
+                    tma_load_2d(a, ma, r, f0, &bar_full[slot]);
+                    if (DUAL) tma_load_2d(a + 16384, &ma1, r, f0, &bar_full[slot]);
+                }
+                if (p.b_mn) {
+                    for (int i = 0; i < p.tn; i += 64) tma_load_2d(b + i * 128, mb, t0 + i, r, &bar_full[slot]);
+                } else {
+                    tma_load_2d(b, mb, r, t0, &bar_full[slot]);
+                }
             }
-            if (p.b_mn) {
-                for (int i = 0; i < p.tn; i += 64) tma_load_2d(b + i * 128, mb, t0 + i, r, &bar_full[slot]);
-            } else {
-                tma_load_2d(b, mb, r, t0, &bar_full[slot]);
-            }
+            __syncwarp();
             if (++slot == p.stages) slot = 0, phase ^= 1;
         }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
         // K-major: rows of 128 bytes, 8-row groups 1024 apart, 16 elements of the reduction 32 bytes on.
         // MN-major: 64-wide panels 8192 apart, 8 steps of the reduction 1024 apart, 16 of them 2048 on.
+        const bool leader = elect_one();
         const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
-        const uint32_t a_lbo = p.a_mn ? 8192 : 16, b_lbo = p.b_mn ? 8192 : 16;
+        const uint64_t ad0 = umma_desc_sw128(smem_u32(base), p.a_mn ? 8192 : 16, 1024);
+        const uint64_t bd0 = umma_desc_sw128(smem_u32(base) + a_bytes, p.b_mn ? 8192 : 16, 1024);
         int slot = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -205,17 +228,19 @@ __global__ void __launch_bounds__(DT_THREADS) dense_tile_kernel(const __grid_con
                 break;
             }
             tc_fence_after();
-            const uint32_t a = smem_u32(base) + (uint32_t)slot * stage_bytes;
-            const uint64_t ad = umma_desc_sw128(a, a_lbo, 1024), bd = umma_desc_sw128(a + a_bytes, b_lbo, 1024);
+            if (leader) {
+                const uint64_t ad = ad0 + (uint64_t)(slot * (stage_bytes >> 4)), bd = bd0 + (uint64_t)(slot * (stage_bytes >> 4));
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                umma_ss(tmem, ad + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
-                if (DUAL) umma_ss(tmem + p.tn, ad + (16384 >> 4) + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
+                for (int k = 0; k < 4; ++k) {
+                    umma_ss(tmem, ad + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
+                    if (DUAL) umma_ss(tmem + p.tn, ad + (16384 >> 4) + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
+                }
+                umma_commit(&bar_free[slot]);
             }
-            umma_commit(&bar_free[slot]);
+            __syncwarp();
             if (++slot == p.stages) slot = 0, phase ^= 1;
         }
-        if (ok) umma_commit(&bar_done);
+        if (ok && leader) umma_commit(&bar_done);
     }
     __syncwarp();
     const bool ok = mbar_wait_abortable(&bar_done, 0, &abort_flag);
@@ -245,11 +270,11 @@ __global__ void __launch_bounds__(DT_THREADS) dense_tile_kernel(const __grid_con
     }
     if (ok) {
         switch (p.act) {
-            case ACT_GELU: dense_epilogue<DUAL, ACT_GELU>(p, tmem, red, f0, t0, group, rank); break;
-            case ACT_SILU: dense_epilogue<DUAL, ACT_SILU>(p, tmem, red, f0, t0, group, rank); break;
-            case ACT_RELU: dense_epilogue<DUAL, ACT_RELU>(p, tmem, red, f0, t0, group, rank); break;
-            case ACT_SIGMOID: dense_epilogue<DUAL, ACT_SIGMOID>(p, tmem, red, f0, t0, group, rank); break;
-            default: dense_epilogue<DUAL, ACT_NONE>(p, tmem, red, f0, t0, group, rank);
+            case ACT_GELU: dense_epilogue<DUAL, ACT_GELU, HALF>(p, tmem, red, f0, t0, group, rank); break;
+            case ACT_SILU: dense_epilogue<DUAL, ACT_SILU, HALF>(p, tmem, red, f0, t0, group, rank); break;
+            case ACT_RELU: dense_epilogue<DUAL, ACT_RELU, HALF>(p, tmem, red, f0, t0, group, rank); break;
+            case ACT_SIGMOID: dense_epilogue<DUAL, ACT_SIGMOID, HALF>(p, tmem, red, f0, t0, group, rank); break;
+            default: dense_epilogue<DUAL, ACT_NONE, HALF>(p, tmem, red, f0, t0, group, rank);
         }
     }
     __syncwarp();
