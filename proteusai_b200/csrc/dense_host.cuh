@@ -68,6 +68,7 @@ static DenseChoice dense_tile_choose(const DenseProduct &d, int sms) {
         const long long tiles = (d.F + DT_FT - 1) / DT_FT * ((d.T + tn - 1) / tn) * d.groups;
         for (int splits = 1; splits <= 8 && splits <= kb; splits *= 2) {
             if (g_dense_tune.kernel == 1 && g_dense_tune.splits && splits != g_dense_tune.splits) continue;
+            if (splits > 1 && tn * acc > 128) continue;  // (the partial rows' buffer)
             const double rounds = (double)((tiles * splits + sms - 1) / sms);
             const double mma = 2.0 * tn * acc, load = (128.0 * acc + tn) * 128.0 / 48.0;
             const double work = (double)((kb + splits - 1) / splits) * (mma > load ? mma : load);
@@ -108,7 +109,7 @@ static DenseChoice dense_choose(const DenseProduct &d, int sms, bool may_split) 
 }
 
 template <bool DUAL, int HALF>
-static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams &p, long long ctas, int smem, cudaStream_t st) {
+static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams &p, dim3 grid, int smem, cudaStream_t st) {
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
@@ -118,7 +119,7 @@ static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)ctas);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(DT_THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
@@ -144,22 +145,23 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
     p.save0 = (float *)d.save[0], p.save1 = (float *)d.save[1];
     p.ld_out = d.ld_out, p.ld_res = d.ld_res;
     p.F = (int)d.F, p.T = (int)d.T;
-    p.f_tiles = (int)((d.F + DT_FT - 1) / DT_FT), p.t_tiles = (int)((d.T + tn - 1) / tn);
-    p.splits = splits, p.tn = tn;
+    const long long f_tiles = (d.F + DT_FT - 1) / DT_FT, t_tiles = (d.T + tn - 1) / tn;  // (f_tiles <= 2^13: widths are limited)
+    p.splits = splits, p.split_log = splits == 8 ? 3 : splits == 4 ? 2 : splits == 2 ? 1 : 0, p.tn = tn;
     p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
     p.a_mn = d.a_mn, p.b_mn = d.b_mn;
     p.act = d.act, p.bias_fp32 = d.bias_fp32;
     p.idesc = dense_idesc(128, tn, d, d.a_mn, d.b_mn);
-    const long long ctas = (long long)p.f_tiles * p.t_tiles * d.groups * splits;
-    if (ctas > 0x7fffffffll) return (int)PAI_ERR_BAD_SHAPE;
+    const long long ctas = f_tiles * t_tiles * d.groups * splits;
+    if (t_tiles * splits > 0x7fffffffll) return (int)PAI_ERR_BAD_SHAPE;
     const int stage = (d.dual ? 2 : 1) * DT_FT * 128 + tn * 128, kb_cta = (p.kb_total + splits - 1) / splits;
-    int stages = (ctas > sms ? 108 * 1024 : 208 * 1024) / stage;
+    const int red = splits > 1 ? tn * DT_FT * 4 * (d.dual ? 2 : 1) : 0;  // partial rows sent here
+    int stages = ((ctas > sms ? 108 : 208) * 1024 - red) / stage;
     stages = stages > DT_MAX_STAGES ? DT_MAX_STAGES : stages;
     stages = stages > kb_cta ? kb_cta : stages;
-    p.stages = stages;
-    int smem = stages * stage;
-    const int red = splits > 1 ? tn * DT_FT * 4 * (d.dual ? 2 : 1) : 0;
-    smem = (smem > red ? smem : red) + 1024;
+    p.stages = stages = stages < 1 ? 1 : stages;
+    // (the stages also hold the CTA's own partial tile)
+    const int smem = (stages * stage > red ? stages * stage : red) + red + 1024;
+    const dim3 grid((unsigned)(t_tiles * splits), (unsigned)f_tiles, d.groups);
     CUtensorMap m[4];
     for (int i = 0; i < 2; ++i) {
         const DenseOperand &a = d.a[i].p ? d.a[i] : d.a[0], &b = d.b[i].p ? d.b[i] : d.b[0];
@@ -168,8 +170,8 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
         if (i == 1 && !d.b[1].p) m[3] = m[2];
         else if (int e = d.b_mn ? make_map_16(&m[2 + i], b.p, d.T, d.R, b.ld, 64, d.half) : make_map_16(&m[2 + i], b.p, d.R, d.T, b.ld, tn, d.half)) return e;
     }
-    if (d.half) return d.dual ? dense_tile_launch_as<true, 1>(m, p, ctas, smem, st) : dense_tile_launch_as<false, 1>(m, p, ctas, smem, st);
-    return d.dual ? dense_tile_launch_as<true, 0>(m, p, ctas, smem, st) : dense_tile_launch_as<false, 0>(m, p, ctas, smem, st);
+    if (d.half) return d.dual ? dense_tile_launch_as<true, 1>(m, p, grid, smem, st) : dense_tile_launch_as<false, 1>(m, p, grid, smem, st);
+    return d.dual ? dense_tile_launch_as<true, 0>(m, p, grid, smem, st) : dense_tile_launch_as<false, 0>(m, p, grid, smem, st);
 }
 
 // map of an operand as MMA rows (`rows` of them, `box` per load): reduction-contiguous or not

@@ -57,11 +57,6 @@ __device__ __forceinline__ uint32_t cluster_ctarank() {
     asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-    return r;
-}
 // Byte offset of the 16-byte chunk `chunk` (0..3) of row `row` inside a [rows x 64 B] tile stored with the 64-byte swizzle.
 __device__ __forceinline__ uint32_t sw64_offset(int row, int chunk) { return (uint32_t)(row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4)); }
 // load into this CTA's shared memory, completion on a barrier of either CTA of the pair (`bar`: shared::cluster address)
