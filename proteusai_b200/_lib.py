@@ -86,6 +86,24 @@ def lib():
     return _lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The PyTorch binding of the feed-forward products (``csrc/torch_ops.cpp``), bound to the entry points of ``lib()``."""
+    global _torch_ops
+    if _torch_ops is None:
+        handle = lib()
+        try:
+            from proteusai_b200 import _torch_ops as module
+        except ImportError as e:
+            raise RuntimeError("proteusai_b200/_torch_ops.so is not there or was built for another PyTorch: build it with "
+                               "`python -m proteusai_b200.build`") from e
+        module.bind({name: ctypes.cast(getattr(handle, name), c_void_p).value for name in SIGNATURES})
+        _torch_ops = module
+    return _torch_ops
+
+
 def check(status, what):
     """Raise RuntimeError for a non-zero status returned by an entry point."""
     if status != 0:

@@ -1,0 +1,272 @@
+// The PyTorch side of the feed-forward products: argument checks, buffers and autograd nodes around the C entry points pai_linear_* and
+// pai_gated_* of libproteus_b200.so, whose addresses the Python loader hands over (bind): this module links no kernel.
+//
+// It is C++ because small products are bound by the host: with autograd nodes in Python a forward + backward of a few microseconds on the GPU took
+// 120 to 200 us, most of it the engine's thread waiting for the interpreter.
+#include <ATen/autocast_mode.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/extension.h>
+
+#include <string>
+
+#include "../../include/proteus_b200.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Api {
+    decltype(&pai_status_str) status_str;
+    decltype(&pai_dense_saved_bytes) saved_bytes;
+    decltype(&pai_dense_bwd_workspace_bytes) workspace_bytes;
+    decltype(&pai_linear_fwd) linear_fwd;
+    decltype(&pai_gated_fwd) gated_fwd;
+    decltype(&pai_linear_bwd) linear_bwd;
+    decltype(&pai_gated_bwd) gated_bwd;
+    decltype(&pai_copy_rows16) copy_rows;
+} api;
+
+void bind(const std::map<std::string, uintptr_t> &at) {
+    auto set = [&](auto &fn, const char *name) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(at.at(name)); };
+    set(api.status_str, "pai_status_str");
+    set(api.saved_bytes, "pai_dense_saved_bytes");
+    set(api.workspace_bytes, "pai_dense_bwd_workspace_bytes");
+    set(api.linear_fwd, "pai_linear_fwd");
+    set(api.gated_fwd, "pai_gated_fwd");
+    set(api.linear_bwd, "pai_linear_bwd");
+    set(api.gated_bwd, "pai_gated_bwd");
+    set(api.copy_rows, "pai_copy_rows16");
+}
+
+void check(int status, const char *what) { TORCH_CHECK(status == 0, what, " failed: ", api.status_str(status), " (status ", status, ")"); }
+
+void *address(const Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
+int dtype_of(const Tensor &t) { return t.scalar_type() == at::kHalf ? PAI_FP16 : PAI_BF16; }
+int is_fp32(const Tensor &b) { return b.defined() && b.scalar_type() == at::kFloat; }
+void *stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
+Tensor bytes(size_t n, const Tensor &like) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte)); }
+
+// t [rows, cols], or a copy, with contiguous columns and rows that do not overlap
+Tensor whole_rows(const Tensor &t) {
+    if ((t.stride(1) == 1 || t.size(1) == 1) && (t.stride(0) >= t.size(1) || t.size(0) == 1)) return t;
+    return t.contiguous();
+}
+
+// t [rows, cols], or a copy, as the products read it: 16-byte aligned rows
+Tensor operand(const Tensor &given) {
+    const Tensor t = whole_rows(given);
+    if (((uintptr_t)t.data_ptr() & 15) == 0 && ((t.stride(0) & 7) == 0 || t.size(0) == 1)) return t;
+    const int64_t rows = t.size(0), cols = t.size(1), pitch = (cols + 7) / 8 * 8;
+    const Tensor out = at::empty({rows, pitch}, t.options());
+    check(api.copy_rows(t.data_ptr(), t.stride(0), out.data_ptr(), pitch, rows, (int)cols, stream()), "pai_copy_rows16");
+    return out.narrow(1, 0, cols);
+}
+
+// y = the product of operands; `saved` receives the pre-activations if wanted.  w2 undefined: linear.
+Tensor forward(const Tensor &x, const Tensor &w, const Tensor &w2, const Tensor &b, const Tensor &b2, const Tensor &r, int act, Tensor *saved) {
+    const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
+    const Tensor y = at::empty({m, n}, x.options());
+    if (m == 0) return y;
+    const bool gated = w2.defined();
+    void *at = nullptr;
+    if (saved && (gated || act != PAI_ACT_NONE)) {
+        *saved = bytes(api.saved_bytes(m, (int)n, (int)k, gated, dtype_of(x)), x);
+        at = saved->data_ptr();
+    }
+    if (gated)
+        check(api.gated_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w2.data_ptr(), w2.stride(0), address(b), address(b2),
+                            is_fp32(b) || is_fp32(b2), y.data_ptr(), n, at, m, (int)n, (int)k, act, dtype_of(x), stream()),
+              "pai_gated_fwd");
+    else
+        check(api.linear_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), address(b), is_fp32(b), address(r), r.defined() ? r.stride(0) : 0,
+                             y.data_ptr(), n, at, m, (int)n, (int)k, act, dtype_of(x), stream()),
+              "pai_linear_fwd");
+    return y;
+}
+
+// a gradient's buffer, if it is wanted (zeros where there are no rows to sum)
+Tensor gradient(bool want, const Tensor &like, at::IntArrayRef shape, bool rows) {
+    if (!want) return Tensor();
+    return rows ? at::empty(shape, like.options()) : at::zeros(shape, like.options());
+}
+
+Tensor or_none(const std::optional<Tensor> &t) { return t.has_value() ? *t : Tensor(); }
+// (autograd's edges count the tensors that are there)
+std::optional<Tensor> maybe(const Tensor &t) { return t.defined() ? std::optional<Tensor>(t) : std::nullopt; }
+
+void first_order_only() {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "fused_ops.linear and gated_linear have first-order gradients only: no create_graph");
+}
+
+struct Linear : torch::autograd::Function<Linear> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &w_, const std::optional<Tensor> &b_, const std::optional<Tensor> &r_,
+                          int64_t act) {
+        const c10::cuda::CUDAGuard guard(x_.device());
+        const Tensor b = or_none(b_), r = or_none(r_);
+        const Tensor x = operand(x_), w = operand(w_);
+        Tensor saved;
+        const bool need = ctx->needs_input_grad(0) || ctx->needs_input_grad(1) || (b.defined() && ctx->needs_input_grad(2));
+        const Tensor y = ::forward(x, w, Tensor(), b, Tensor(), r, (int)act, need ? &saved : nullptr);
+        ctx->save_for_backward({x, w, b, saved});
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["edges"] = (int64_t)(b.defined() ? 1 : 0) | (int64_t)(r.defined() ? 2 : 0);
+        return y;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const Tensor &dy = grads[0];
+        const int64_t edges = ctx->saved_data["edges"].toInt();
+        const bool has_b = edges & 1, has_r = edges & 2;
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1), need_b = has_b && ctx->needs_input_grad(2);
+        const Tensor dr = has_r && ctx->needs_input_grad(has_b ? 3 : 2) ? dy : Tensor();
+        if (!dy.defined() || !(need_x || need_w || need_b)) return {Tensor(), Tensor(), Tensor(), dr, Tensor()};
+        first_order_only();
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &w = saved[1], &b = saved[2];
+        const c10::cuda::CUDAGuard guard(x.device());
+        const int64_t m = x.size(0), k = x.size(1), n = w.size(0), act = ctx->saved_data["act"].toInt();
+        const Tensor dx = gradient(need_x, x, {m, k}, true), dw = gradient(need_w, w, {n, k}, m > 0), db = gradient(need_b, b, {n}, m > 0);
+        if (m > 0) {
+            const Tensor d = act == PAI_ACT_NONE && (need_x || need_w) ? operand(dy) : whole_rows(dy);
+            const size_t size = api.workspace_bytes(m, (int)n, (int)k, 0);
+            const Tensor ws = bytes(size, x);
+            check(api.linear_bwd(d.data_ptr(), d.stride(0), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), address(saved[3]), address(dx), k,
+                                 address(dw), address(db), is_fp32(b), ws.data_ptr(), size, m, (int)n, (int)k, (int)act, dtype_of(x), stream()),
+                  "pai_linear_bwd");
+        }
+        return {dx, dw, db, dr, Tensor()};
+    }
+};
+
+struct Gated : torch::autograd::Function<Gated> {
+    static Tensor forward(AutogradContext *ctx, const Tensor &x_, const Tensor &wg_, const Tensor &wu_, const std::optional<Tensor> &bg_,
+                          const std::optional<Tensor> &bu_, int64_t act) {
+        const c10::cuda::CUDAGuard guard(x_.device());
+        const Tensor bg = or_none(bg_), bu = or_none(bu_);
+        const Tensor x = operand(x_), wg = operand(wg_), wu = wu_.is_same(wg_) ? wg : operand(wu_);
+        Tensor saved;
+        const Tensor h = ::forward(x, wg, wu, bg, bu, Tensor(), (int)act, &saved);
+        ctx->save_for_backward({x, wg, wu, bg, bu, saved});
+        ctx->saved_data["act"] = act;
+        return h;
+    }
+    static variable_list backward(AutogradContext *ctx, variable_list grads) {
+        const Tensor &dh = grads[0];
+        if (!dh.defined()) return variable_list(6);
+        first_order_only();
+        const variable_list saved = ctx->get_saved_variables();
+        const Tensor &x = saved[0], &wg = saved[1], &wu = saved[2], &bg = saved[3], &bu = saved[4];
+        const c10::cuda::CUDAGuard guard(x.device());
+        const int64_t m = x.size(0), k = x.size(1), n = wg.size(0), act = ctx->saved_data["act"].toInt();
+        const Tensor dx = gradient(ctx->needs_input_grad(0), x, {m, k}, true);
+        const Tensor dwg = gradient(ctx->needs_input_grad(1), wg, {n, k}, m > 0), dwu = gradient(ctx->needs_input_grad(2), wu, {n, k}, m > 0);
+        const Tensor dbg = gradient(bg.defined() && ctx->needs_input_grad(3), bg, {n}, m > 0);
+        const Tensor dbu = gradient(bu.defined() && ctx->needs_input_grad(bg.defined() ? 4 : 3), bu, {n}, m > 0);
+        if (m > 0) {
+            const Tensor d = whole_rows(dh);
+            const size_t size = api.workspace_bytes(m, (int)n, (int)k, 1);
+            const Tensor ws = bytes(size, x);
+            check(api.gated_bwd(d.data_ptr(), d.stride(0), x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0),
+                                address(saved[5]), address(dx), k, address(dwg), address(dwu), address(dbg), address(dbu), is_fp32(bg) || is_fp32(bu),
+                                ws.data_ptr(), size, m, (int)n, (int)k, (int)act, dtype_of(x), stream()),
+                  "pai_gated_bwd");
+        }
+        return {dx, dwg, dwu, dbg, dbu, Tensor()};
+    }
+};
+
+// ---- arguments --------------------------------------------------------------------------------------------------------
+bool given(const Tensor &t) { return t.defined(); }
+
+// The checks both operators share (undefined: left out); ws: one or two weights.
+void check_arguments(const char *what, const Tensor &x, at::ArrayRef<Tensor> ws, at::ArrayRef<Tensor> bs, const Tensor &r) {
+    for (const auto &list : {at::ArrayRef<Tensor>(x), ws, bs, at::ArrayRef<Tensor>(r)})
+        for (const Tensor &t : list) TORCH_CHECK(!given(t) || t.is_cuda(), what, " needs CUDA tensors: there is no CPU path");
+    for (const auto &list : {ws, bs, at::ArrayRef<Tensor>(r)})
+        for (const Tensor &t : list) TORCH_CHECK(!given(t) || t.device() == x.device(), what, ": all tensors must be on one device");
+    const auto dt = x.scalar_type();
+    for (const Tensor &w : ws)
+        TORCH_CHECK_TYPE((dt == at::kBFloat16 || dt == at::kHalf) && w.scalar_type() == dt, what,
+                         ": x and weights must all be bfloat16 or all float16, not ", dt, " and ", w.scalar_type());
+    for (const Tensor &w : ws)
+        TORCH_CHECK_VALUE(x.dim() >= 1 && w.dim() == 2 && w.sizes() == ws[0].sizes() && w.size(1) == x.size(-1), what,
+                          ": x [..., d_in] and weights [d_out, d_in] do not fit: ", x.sizes(), " and ", w.sizes());
+    TORCH_CHECK_VALUE(ws[0].size(0) > 0 && ws[0].size(1) > 0, what, ": weights must not be empty: ", ws[0].sizes());
+    const Tensor *first = nullptr;
+    for (const Tensor &b : bs)
+        if (given(b)) {
+            if (!first) first = &b;
+            TORCH_CHECK_VALUE(b.dim() == 1 && b.size(0) == ws[0].size(0), what, ": a bias must have shape [", ws[0].size(0), "], not ", b.sizes());
+            TORCH_CHECK_TYPE((b.scalar_type() == dt || b.scalar_type() == at::kFloat) && b.scalar_type() == first->scalar_type(), what,
+                             ": biases must all be ", dt, " or all float32, not ", b.scalar_type());
+        }
+    if (given(r)) {
+        TORCH_CHECK_TYPE(r.scalar_type() == dt, what, ": residual must be ", dt, ", not ", r.scalar_type());
+        bool same = r.dim() == x.dim() && r.size(-1) == ws[0].size(0);
+        for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = r.size(i) == x.size(i);
+        TORCH_CHECK_VALUE(same, what, ": residual must have the output's shape, x's with ", ws[0].size(0), " columns; got ", r.sizes(), " beside ",
+                          x.sizes());
+    }
+}
+
+Tensor cast(const Tensor &t, at::ScalarType dt, bool keep_fp32 = false) {
+    return !given(t) || t.scalar_type() == dt || !t.is_floating_point() || (keep_fp32 && t.scalar_type() == at::kFloat) ? t : t.to(dt);
+}
+bool autocast() { return at::autocast::is_autocast_enabled(at::kCUDA); }
+Tensor flat(const Tensor &t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+Tensor shaped(const Tensor &y, const Tensor &x) {
+    if (x.dim() == 2) return y;
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = y.size(1);
+    return y.view(shape);
+}
+Tensor contiguous(const Tensor &b) { return given(b) ? b.contiguous() : b; }
+bool recording(std::initializer_list<Tensor> ts) {
+    if (!at::GradMode::is_enabled()) return false;
+    for (const Tensor &t : ts)
+        if (given(t) && t.requires_grad()) return true;
+    return false;
+}
+Tensor linear(Tensor x, Tensor w, const std::optional<Tensor> &b_, int64_t act, const std::optional<Tensor> &r_) {
+    Tensor b = or_none(b_), r = or_none(r_);
+    if (autocast()) {
+        const auto dt = at::autocast::get_autocast_dtype(at::kCUDA);
+        x = cast(x, dt), w = cast(w, dt), b = cast(b, dt, true), r = cast(r, dt);
+    }
+    check_arguments("linear", x, w, b, r);
+    b = contiguous(b);
+    const Tensor x2 = flat(x);
+    if (given(r)) {
+        r = flat(r);
+        if (r.stride(1) != 1 && r.size(1) != 1) r = r.contiguous();
+    }
+    if (recording({x2, w, b, r})) return shaped(Linear::apply(x2, w, maybe(b), maybe(r), act), x);
+    const c10::cuda::CUDAGuard guard(x.device());
+    return shaped(forward(operand(x2), operand(w), Tensor(), b, Tensor(), r, (int)act, nullptr), x);
+}
+
+Tensor gated_linear(Tensor x, Tensor wg, Tensor wu, const std::optional<Tensor> &bg_, const std::optional<Tensor> &bu_, int64_t act) {
+    Tensor bg = or_none(bg_), bu = or_none(bu_);
+    if (autocast()) {
+        const auto dt = at::autocast::get_autocast_dtype(at::kCUDA);
+        x = cast(x, dt), wg = cast(wg, dt), wu = cast(wu, dt), bg = cast(bg, dt, true), bu = cast(bu, dt, true);
+    }
+    check_arguments("gated_linear", x, {wg, wu}, {bg, bu}, Tensor());
+    bg = contiguous(bg), bu = contiguous(bu);
+    const Tensor x2 = flat(x);
+    if (recording({x2, wg, wu, bg, bu})) return shaped(Gated::apply(x2, wg, wu, maybe(bg), maybe(bu), act), x);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor a = operand(wg);
+    return shaped(forward(operand(x2), a, wu.is_same(wg) ? a : operand(wu), bg, bu, Tensor(), (int)act, nullptr), x);
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_torch_ops, m) {
+    m.def("bind", &bind);
+    m.def("linear", &linear, pybind11::call_guard<pybind11::gil_scoped_release>());
+    m.def("gated_linear", &gated_linear, pybind11::call_guard<pybind11::gil_scoped_release>());
+}
