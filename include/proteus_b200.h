@@ -406,7 +406,7 @@ enum pai_tune_key {
     PAI_TUNE_GA_NO_ORDER = 7,     /* 1: issue the samples in natural order instead of longest first */
     PAI_TUNE_WE_MIXED = 8,        /* 1: separate SFU and polynomial warps (we_fwd_mixed_kernel) instead of both pipes in every warp;
                                      measured 12 % slower at N = 16384, kept for comparison (default 0) */
-    PAI_TUNE_DENSE_KERNEL = 9,    /* feed-forward products: 1 = dense_tile_kernel, 2 = dense_pair_kernel (set it before the forward call and leave
+    PAI_TUNE_DENSE_KERNEL = 9,    /* feed-forward products: 1 = dense_tile_kernel, 2 = dense_pair_kernel, 3 = dense_vec_kernel where it applies (set it before the forward call and leave
                                      it until the backward call has been made: the saved pre-activations go by the kernel) */
     PAI_TUNE_DENSE_WIDTH = 10,    /* with it: rows of a tile (16 .. 256), accumulator columns of a pair's tile (128, 256) */
     PAI_TUNE_DENSE_SPLITS = 11,   /* with it: split of the reduction (tile: 1, 2, 4, 8; pair: weight gradients only, 1 .. 16) */

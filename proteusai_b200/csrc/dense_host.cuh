@@ -2,6 +2,7 @@
 #pragma once
 #include "dense_pair.cuh"
 #include "dense_tile.cuh"
+#include "dense_vec.cuh"
 
 namespace pai {
 
@@ -44,7 +45,7 @@ struct DenseProduct {
     float *part;               // workspace of a split reduction in the pair kernel (dense_pair_choose), or NULL: no split
 };
 
-// Test-only overrides of the choices below (0: none): kernel 1 = tile, 2 = pair; tile height / accumulator columns; split.
+// Test-only overrides of the choices below (0: none): kernel 1 = tile, 2 = pair (3 = vec, which takes no shape); tile height / accumulator columns; split.
 struct DenseTune {
     int kernel, width, splits;
 };
@@ -104,7 +105,7 @@ static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_sp
 
 static DenseChoice dense_choose(const DenseProduct &d, int sms, bool may_split) {
     const DenseChoice a = dense_tile_choose(d, sms), b = dense_pair_choose(d, sms, may_split);
-    if (g_dense_tune.kernel) return g_dense_tune.kernel == 2 ? b : a;
+    if (g_dense_tune.kernel) return g_dense_tune.kernel == 2 ? b : a;  // (3: what the vec kernel does not run)
     return b.cost < a.cost ? b : a;
 }
 
@@ -254,6 +255,45 @@ static int dense_launch(const DenseProduct &d, int sms, cudaStream_t st) {
     return c.pair ? dense_pair_launch(d, c, sms, st) : dense_tile_launch(d, c, sms, st);
 }
 
+// ---- up to eight tokens ---------------------------------------------------------------------------------------------
+template <bool DUAL, int ACT, int TT>
+static void dense_vec_as(const DenseVecParams &p, int half, unsigned grid, cudaStream_t st) {
+    if (half) dense_vec_kernel<DUAL, ACT, TT, 1><<<grid, DV_WARPS * 32, 0, st>>>(p);
+    else dense_vec_kernel<DUAL, ACT, TT, 0><<<grid, DV_WARPS * 32, 0, st>>>(p);
+}
+template <bool DUAL, int ACT>
+static void dense_vec_tokens(const DenseVecParams &p, int half, unsigned grid, cudaStream_t st) {
+    if (p.T <= 1) dense_vec_as<DUAL, ACT, 1>(p, half, grid, st);
+    else if (p.T <= 2) dense_vec_as<DUAL, ACT, 2>(p, half, grid, st);
+    else if (p.T <= 4) dense_vec_as<DUAL, ACT, 4>(p, half, grid, st);
+    else dense_vec_as<DUAL, ACT, 8>(p, half, grid, st);
+}
+template <bool DUAL>
+static int dense_vec_act(const DenseVecParams &p, int act, int half, cudaStream_t st) {
+    const int per_cta = DV_WARPS * (DUAL ? 1 : 2);
+    const unsigned grid = (unsigned)((p.N + per_cta - 1) / per_cta);
+    switch (act) {
+        case ACT_GELU: dense_vec_tokens<DUAL, ACT_GELU>(p, half, grid, st); break;
+        case ACT_SILU: dense_vec_tokens<DUAL, ACT_SILU>(p, half, grid, st); break;
+        case ACT_RELU: dense_vec_tokens<DUAL, ACT_RELU>(p, half, grid, st); break;
+        case ACT_SIGMOID: dense_vec_tokens<DUAL, ACT_SIGMOID>(p, half, grid, st); break;
+        default: dense_vec_tokens<DUAL, ACT_NONE>(p, half, grid, st);
+    }
+    return (int)cudaPeekAtLastError();
+}
+static bool dense_uses_vec(long long T) { return T <= DV_MAX_TOKENS && (g_dense_tune.kernel == 0 || g_dense_tune.kernel == 3); }
+static int dense_vec_launch(const DenseProduct &d, cudaStream_t st) {
+    DenseVecParams p = {};
+    p.x = (const unsigned short *)d.b[0].p, p.w0 = (const unsigned short *)d.a[0].p, p.w1 = (const unsigned short *)d.a[1].p;
+    p.ld_x = d.b[0].ld, p.ld_w0 = d.a[0].ld, p.ld_w1 = d.a[1].ld;
+    p.bias0 = d.bias[0], p.bias1 = d.bias[1], p.bias_fp32 = d.bias_fp32;
+    p.residual = (const unsigned short *)d.residual, p.ld_res = d.ld_res;
+    p.out = (unsigned short *)d.out[0], p.ld_out = d.ld_out;
+    p.save0 = (float *)d.save[0], p.save1 = (float *)d.save[1];
+    p.T = (int)d.T, p.N = (int)d.F, p.K = (int)d.R;
+    return d.dual ? dense_vec_act<true>(p, d.act, d.half, st) : dense_vec_act<false>(p, d.act, d.half, st);
+}
+
 // The products as problems (sizes only): what the saved buffer and the workspace are sized for, and what runs.
 static DenseProduct dense_forward_product(long long M, int N, int K, int gated) {
     DenseProduct d = {};
@@ -269,7 +309,7 @@ static DenseProduct dense_weight_product(long long M, int N, int K, int groups) 
 }
 // the form of the saved pre-activations: fp16 with exponents where the pair kernel runs on bf16, fp32 otherwise
 static bool dense_saves_f32(long long M, int N, int K, int gated, int half, int sms) {
-    return half || !dense_choose(dense_forward_product(M, N, K, gated), sms, false).pair;
+    return half || dense_uses_vec(M) || !dense_choose(dense_forward_product(M, N, K, gated), sms, false).pair;
 }
 static size_t dense_saved_matrix(long long M, int N, int K, int gated, int half, int sms) {
     return dense_saves_f32(M, N, K, gated, half, sms) ? saved_bytes_f32(M, N) : saved_bytes_f16(M, N);
@@ -288,7 +328,7 @@ static int dense_forward(const DenseOperand &x, const DenseOperand (&w)[2], cons
     d.save[0] = saved;
     d.save[1] = saved && gated ? (char *)saved + dense_saved_matrix(M, N, K, gated, half, sms) : nullptr;
     d.act = act, d.half = half;
-    return dense_launch(d, sms, st);
+    return dense_uses_vec(M) ? dense_vec_launch(d, st) : dense_launch(d, sms, st);
 }
 
 // Strips of the elementwise pass: about four CTAs of 256 threads per SM, at least 64 rows each.

@@ -21,7 +21,7 @@ pytestmark = pytest.mark.gpu
 ACTS = (None, "gelu", "silu", "relu", "sigmoid")
 DTYPES = (torch.bfloat16, torch.float16)
 # rows, d_in, d_out: single tokens, single columns, odd widths, tile borders (16, 32, 64, 128, 256 rows; 64 and 128 columns), ragged batches
-SHAPES = [(1, 1, 1), (1, 512, 2048), (2, 8, 16), (3, 7, 5), (16, 64, 128), (17, 65, 129), (33, 1000, 20), (64, 130, 66), (131, 512, 1024),
+SHAPES = [(1, 1, 1), (1, 512, 2048), (2, 8, 16), (3, 7, 5), (4, 2056, 33), (8, 300, 77), (9, 300, 77), (16, 64, 128), (17, 65, 129), (33, 1000, 20), (64, 130, 66), (131, 512, 1024),
           (256, 2048, 512), (300, 96, 1), (777, 250, 1023), (1025, 72, 136)]
 
 
