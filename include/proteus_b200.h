@@ -324,8 +324,8 @@ int pai_gelu_bf16(const void *x, void *out, long long n, void *stream);
  *              in a layout of the library's own; pai_linear_bwd without an activation needs none.
  *   workspace  pai_dense_bwd_workspace_bytes(M, N, K, gated) bytes, 256-byte aligned.
  * Limits: M < 2^31 - 2^16, N and K <= 2^20.  Results are the same bits from call to call.
- *   pai_copy_rows16  dst[r, c] = src[r, c] for rows of 16-bit elements of any alignment into 16-byte aligned rows; columns up to the next
- *                    multiple of 8 are written as zeros.
+ *   pai_copy_rows16  dst[i][r, c] = src[i][r, c] for `count` (1 to 3) matrices with rows of 16-bit elements of any alignment into 16-byte
+ *                    aligned rows, in one launch; columns up to the next multiple of 8 are written as zeros.  The arrays are host memory.
  */
 enum pai_dtype { PAI_BF16 = 0, PAI_FP16 = 1 };
 enum pai_act { PAI_ACT_NONE = 0, PAI_ACT_GELU = 1 /* erf form */, PAI_ACT_SILU = 2, PAI_ACT_RELU = 3, PAI_ACT_SIGMOID = 4 };
@@ -343,7 +343,8 @@ int pai_linear_bwd(const void *dy, int64_t lddy, const void *x, int64_t ldx, con
 int pai_gated_bwd(const void *dh, int64_t lddh, const void *x, int64_t ldx, const void *w_gate, int64_t ldwg, const void *w_up, int64_t ldwu,
                   const void *saved, void *dx, int64_t lddx, void *dw_gate, void *dw_up, void *db_gate, void *db_up, int bias_fp32, void *workspace,
                   size_t workspace_bytes, long long M, int N, int K, int act, int dtype, void *stream);
-int pai_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld_dst, long long rows, int cols, void *stream);
+int pai_copy_rows16(int count, const void *const *src, const int64_t *ld_src, void *const *dst, const int64_t *ld_dst, const long long *rows,
+                    const int *cols, void *stream);
 
 /* ---------------------------------------------------------------------------------------
  * Nearest-neighbour graph and radial-basis edge features: FeaturizeProtein.get_neighbors and the tensor part of

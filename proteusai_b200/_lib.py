@@ -51,7 +51,7 @@ SIGNATURES = {
                                c_void_p, c_size_t, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "pai_gated_bwd": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64,
                               c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_size_t, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
-    "pai_copy_rows16": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p]),
+    "pai_copy_rows16": (c_int, [c_int] + [c_void_p] * 7),
     "pai_knn_neighbors": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_float, c_void_p]),
     "pai_edge_rbf": (c_int, [c_void_p, c_void_p, c_void_p, c_double, c_void_p, c_void_p, c_float, c_void_p,
                              c_int, c_int, c_int, c_int, c_int, c_void_p]),

@@ -750,17 +750,24 @@ int pai_gated_bwd(const void *dh, int64_t lddh, const void *x, int64_t ldx, cons
                                (cudaStream_t)stream);
 }
 
-int pai_copy_rows16(const void *src, int64_t ld_src, void *dst, int64_t ld_dst, long long rows, int cols, void *stream) {
-    if (rows < 0 || rows > PAI_DENSE_MAX_ROWS || cols < 1 || cols > PAI_DENSE_MAX_WIDTH) return PAI_ERR_BAD_SHAPE;
-    if (int e = check_dense_rows(src, ld_src, rows, cols, false)) return e;
-    if (!dst) return PAI_ERR_NULL_POINTER;
-    if (ld_dst < pai::dense_ld16(cols)) return PAI_ERR_BAD_SHAPE;
-    if (!aligned(dst, 16) || (ld_dst & 7) != 0) return PAI_ERR_MISALIGNED;
+int pai_copy_rows16(int count, const void *const *src, const int64_t *ld_src, void *const *dst, const int64_t *ld_dst, const long long *rows,
+                    const int *cols, void *stream) {
+    if (!src || !ld_src || !dst || !ld_dst || !rows || !cols) return PAI_ERR_NULL_POINTER;
+    if (count < 1 || count > pai::DENSE_MAX_COPIES) return PAI_ERR_BAD_SHAPE;
+    pai::DenseCopyParams p = {};
+    for (int i = 0; i < count; ++i) {
+        if (rows[i] < 0 || rows[i] > PAI_DENSE_MAX_ROWS || cols[i] < 1 || cols[i] > PAI_DENSE_MAX_WIDTH) return PAI_ERR_BAD_SHAPE;
+        if (int e = check_dense_rows(src[i], ld_src[i], rows[i], cols[i], false)) return e;
+        if (!dst[i]) return PAI_ERR_NULL_POINTER;
+        if (ld_dst[i] < pai::dense_ld16(cols[i])) return PAI_ERR_BAD_SHAPE;
+        if (!aligned(dst[i], 16) || (ld_dst[i] & 7) != 0) return PAI_ERR_MISALIGNED;
+        p.src[i] = (const unsigned short *)src[i], p.dst[i] = (unsigned short *)dst[i];
+        p.ld_src[i] = ld_src[i], p.ld_dst[i] = ld_dst[i], p.rows[i] = rows[i], p.cols[i] = cols[i];
+    }
     if (int e = require_sm100()) return e;
-    if (rows == 0) return PAI_OK;
     int sms = 0;
     if (int e = current_device_sms(&sms)) return e;
-    return pai::dense_copy_rows(src, ld_src, dst, ld_dst, rows, cols, sms, (cudaStream_t)stream);
+    return pai::dense_copy_rows(p, count, sms, (cudaStream_t)stream);
 }
 
 int pai_knn_neighbors(const float *ca, const uint8_t *valid, int64_t *idx, uint8_t *edge_mask, int Z, int N, int K, float max_dist,

@@ -444,11 +444,13 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
     return 0;
 }
 
-static int dense_copy_rows(const void *src, long long ld_src, void *dst, long long ld_dst, long long rows, int cols, int sms, cudaStream_t st) {
-    const long long n = rows * ((cols + 7) / 8);
-    long long blocks = (n + 255) / 256;
-    if (blocks > (long long)sms * 32) blocks = (long long)sms * 32;
-    dense_copy_rows_kernel<<<(unsigned)blocks, 256, 0, st>>>((const unsigned short *)src, ld_src, (unsigned short *)dst, ld_dst, rows, cols);
+static int dense_copy_rows(const DenseCopyParams &p, int count, int sms, cudaStream_t st) {
+    long long most = 0;
+    for (int i = 0; i < count; ++i) most = p.rows[i] * ((p.cols[i] + 7) / 8) > most ? p.rows[i] * ((p.cols[i] + 7) / 8) : most;
+    if (most == 0) return 0;
+    long long blocks = (most + 255) / 256;
+    if (blocks > (long long)sms * 16) blocks = (long long)sms * 16;
+    dense_copy_rows_kernel<<<dim3((unsigned)blocks, count), 256, 0, st>>>(p);
     return (int)cudaPeekAtLastError();
 }
 

@@ -291,22 +291,28 @@ __global__ void __launch_bounds__(256) dense_colsum_kernel(const float *__restri
     }
 }
 
-// dst[r, 0 .. cols) = src[r, 0 .. cols) for rows of any alignment: TMA wants 16-byte aligned rows
-__global__ void __launch_bounds__(256) dense_copy_rows_kernel(const unsigned short *__restrict__ src, long long ld_src, unsigned short *__restrict__ dst,
-                                                              long long ld_dst, long long rows, int cols) {
-    const int words = (cols + 7) >> 3;
-    const long long n = rows * words, stride = (long long)gridDim.x * 256;
+// dst[r, 0 .. cols) = src[r, 0 .. cols) for rows of any alignment (TMA wants 16-byte aligned ones), up to three matrices in a launch
+constexpr int DENSE_MAX_COPIES = 3;
+struct DenseCopyParams {
+    const unsigned short *src[DENSE_MAX_COPIES];
+    unsigned short *dst[DENSE_MAX_COPIES];
+    long long ld_src[DENSE_MAX_COPIES], ld_dst[DENSE_MAX_COPIES], rows[DENSE_MAX_COPIES];
+    int cols[DENSE_MAX_COPIES];
+};
+__global__ void __launch_bounds__(256) dense_copy_rows_kernel(const __grid_constant__ DenseCopyParams p) {
+    const int m = blockIdx.y, cols = p.cols[m], words = (cols + 7) >> 3;
+    const long long n = p.rows[m] * words, stride = (long long)gridDim.x * 256;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {
         const long long r = i / words;
         const int c = (int)(i - r * words) * 8;
-        const unsigned short *s = src + r * ld_src + c;
+        const unsigned short *s = p.src[m] + r * p.ld_src[m] + c;
         uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const uint32_t lo = c + 2 * k < cols ? s[2 * k] : 0, hi = c + 2 * k + 1 < cols ? s[2 * k + 1] : 0;
             w[k] = lo | hi << 16;
         }
-        *reinterpret_cast<uint4 *>(dst + r * ld_dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(p.dst[m] + r * p.ld_dst[m] + c) = make_uint4(w[0], w[1], w[2], w[3]);
     }
 }
 

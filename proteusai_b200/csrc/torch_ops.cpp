@@ -56,34 +56,64 @@ Tensor whole_rows(const Tensor &t) {
     return t.contiguous();
 }
 
-// t [rows, cols], or a copy, as the products read it: 16-byte aligned rows
-Tensor operand(const Tensor &given) {
-    const Tensor t = whole_rows(given);
-    if (((uintptr_t)t.data_ptr() & 15) == 0 && ((t.stride(0) & 7) == 0 || t.size(0) == 1)) return t;
-    const int64_t rows = t.size(0), cols = t.size(1), pitch = (cols + 7) / 8 * 8;
-    const Tensor out = at::empty({rows, pitch}, t.options());
-    check(api.copy_rows(t.data_ptr(), t.stride(0), out.data_ptr(), pitch, rows, (int)cols, stream()), "pai_copy_rows16");
-    return out.narrow(1, 0, cols);
-}
+// The products' operands as they are read: 16-byte aligned rows.  Those whose rows are not (odd widths, odd offsets) lie as copies in `copies`, one
+// buffer and one launch for all; `copies` of the forward pass serves the backward pass.
+struct Operands {
+    const void *p[3];
+    int64_t ld[3];
+    Tensor copies;
 
-// y = the product of operands; `saved` receives the pre-activations if wanted.  w2 undefined: linear.
-Tensor forward(const Tensor &x, const Tensor &w, const Tensor &w2, const Tensor &b, const Tensor &b2, const Tensor &r, int act, Tensor *saved) {
-    const int64_t m = x.size(0), k = x.size(1), n = w.size(0);
+    Operands(std::initializer_list<Tensor> ts, const Tensor &kept = Tensor()) : copies(kept) {
+        const void *src[3];
+        void *dst[3];
+        int64_t ld_src[3], ld_dst[3];
+        long long rows[3];
+        int cols[3], n = 0, i = 0;
+        int64_t elements = 0;
+        for (const Tensor &t : ts) {
+            p[i] = t.defined() ? t.data_ptr() : nullptr, ld[i] = t.defined() ? t.stride(0) : 0;
+            if (t.defined() && t.size(0) > 0 && (((uintptr_t)p[i] & 15) != 0 || ((ld[i] & 7) != 0 && t.size(0) > 1))) {
+                src[n] = p[i], ld_src[n] = ld[i], rows[n] = t.size(0), cols[n] = (int)t.size(1);
+                ld_dst[n] = (t.size(1) + 7) / 8 * 8;
+                dst[n] = reinterpret_cast<void *>(elements * 2);  // (offset until the buffer is there)
+                p[i] = nullptr, ld[i] = n++;
+                elements += t.size(0) * ld_dst[n - 1];
+            }
+            ++i;
+        }
+        if (n == 0) return;
+        const bool fill = !copies.defined();
+        if (fill) copies = at::empty({elements}, ts.begin()->options());
+        for (int k = 0; k < n; ++k) dst[k] = (char *)copies.data_ptr() + (size_t)dst[k];
+        i = 0;
+        for (const Tensor &t : ts) {
+            if (t.defined() && t.size(0) > 0 && !p[i]) {
+                const int k = (int)ld[i];
+                p[i] = dst[k], ld[i] = ld_dst[k];
+            }
+            ++i;
+        }
+        if (fill) check(api.copy_rows(n, src, ld_src, dst, ld_dst, rows, cols, stream()), "pai_copy_rows16");
+    }
+};
+
+// y [m, n] from x [m, k] and w [n, k] (o: their operands); `saved` receives the pre-activations if wanted.  Gated: o.p[2] is the second weight.
+Tensor forward(const Operands &o, const Tensor &x, int64_t n, bool gated, const Tensor &b, const Tensor &b2, const Tensor &r, int act, Tensor *saved) {
+    const int64_t m = x.size(0), k = x.size(1);
     const Tensor y = at::empty({m, n}, x.options());
     if (m == 0) return y;
-    const bool gated = w2.defined();
     void *at = nullptr;
     if (saved && (gated || act != PAI_ACT_NONE)) {
         *saved = bytes(api.saved_bytes(m, (int)n, (int)k, gated, dtype_of(x)), x);
         at = saved->data_ptr();
     }
     if (gated)
-        check(api.gated_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), w2.data_ptr(), w2.stride(0), address(b), address(b2),
-                            is_fp32(b) || is_fp32(b2), y.data_ptr(), n, at, m, (int)n, (int)k, act, dtype_of(x), stream()),
+        check(api.gated_fwd(o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], address(b), address(b2), is_fp32(b) || is_fp32(b2), y.data_ptr(), n, at,
+                            m, (int)n, (int)k, act, dtype_of(x), stream()),
               "pai_gated_fwd");
     else
-        check(api.linear_fwd(x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), address(b), is_fp32(b), address(r), r.defined() ? r.stride(0) : 0,
-                             y.data_ptr(), n, at, m, (int)n, (int)k, act, dtype_of(x), stream()),
+        check(api.linear_fwd(o.p[0], o.ld[0], o.p[1], o.ld[1], address(b), is_fp32(b), address(r), r.defined() ? r.stride(0) : 0, y.data_ptr(), n, at,
+                             m, (int)n, (int)k, act, dtype_of(x), stream()),
               "pai_linear_fwd");
     return y;
 }
@@ -107,11 +137,12 @@ struct Linear : torch::autograd::Function<Linear> {
                           int64_t act) {
         const c10::cuda::CUDAGuard guard(x_.device());
         const Tensor b = or_none(b_), r = or_none(r_);
-        const Tensor x = operand(x_), w = operand(w_);
+        const Tensor x = whole_rows(x_), w = whole_rows(w_);
+        const Operands o({x, w});
         Tensor saved;
         const bool need = ctx->needs_input_grad(0) || ctx->needs_input_grad(1) || (b.defined() && ctx->needs_input_grad(2));
-        const Tensor y = ::forward(x, w, Tensor(), b, Tensor(), r, (int)act, need ? &saved : nullptr);
-        ctx->save_for_backward({x, w, b, saved});
+        const Tensor y = ::forward(o, x, w.size(0), false, b, Tensor(), r, (int)act, need ? &saved : nullptr);
+        ctx->save_for_backward({x, w, b, saved, o.copies});
         ctx->saved_data["act"] = act;
         ctx->saved_data["edges"] = (int64_t)(b.defined() ? 1 : 0) | (int64_t)(r.defined() ? 2 : 0);
         return y;
@@ -130,10 +161,14 @@ struct Linear : torch::autograd::Function<Linear> {
         const int64_t m = x.size(0), k = x.size(1), n = w.size(0), act = ctx->saved_data["act"].toInt();
         const Tensor dx = gradient(need_x, x, {m, k}, true), dw = gradient(need_w, w, {n, k}, m > 0), db = gradient(need_b, b, {n}, m > 0);
         if (m > 0) {
-            const Tensor d = act == PAI_ACT_NONE && (need_x || need_w) ? operand(dy) : whole_rows(dy);
+            const Operands o({x, w}, saved[4]);
+            const Tensor d = whole_rows(dy);
+            const bool product = act == PAI_ACT_NONE && (need_x || need_w);  // dy itself is an operand
+            const Operands od({product ? d : Tensor()});
             const size_t size = api.workspace_bytes(m, (int)n, (int)k, 0);
             const Tensor ws = bytes(size, x);
-            check(api.linear_bwd(d.data_ptr(), d.stride(0), x.data_ptr(), x.stride(0), w.data_ptr(), w.stride(0), address(saved[3]), address(dx), k,
+            check(api.linear_bwd(product ? od.p[0] : d.data_ptr(), product ? od.ld[0] : d.stride(0), o.p[0], o.ld[0], o.p[1], o.ld[1], address(saved[3]),
+                                 address(dx), k,
                                  address(dw), address(db), is_fp32(b), ws.data_ptr(), size, m, (int)n, (int)k, (int)act, dtype_of(x), stream()),
                   "pai_linear_bwd");
         }
@@ -146,10 +181,11 @@ struct Gated : torch::autograd::Function<Gated> {
                           const std::optional<Tensor> &bu_, int64_t act) {
         const c10::cuda::CUDAGuard guard(x_.device());
         const Tensor bg = or_none(bg_), bu = or_none(bu_);
-        const Tensor x = operand(x_), wg = operand(wg_), wu = wu_.is_same(wg_) ? wg : operand(wu_);
+        const Tensor x = whole_rows(x_), wg = whole_rows(wg_), wu = whole_rows(wu_);
+        const Operands o({x, wg, wu});
         Tensor saved;
-        const Tensor h = ::forward(x, wg, wu, bg, bu, Tensor(), (int)act, &saved);
-        ctx->save_for_backward({x, wg, wu, bg, bu, saved});
+        const Tensor h = ::forward(o, x, wg.size(0), true, bg, bu, Tensor(), (int)act, &saved);
+        ctx->save_for_backward({x, wg, wu, bg, bu, saved, o.copies});
         ctx->saved_data["act"] = act;
         return h;
     }
@@ -166,11 +202,11 @@ struct Gated : torch::autograd::Function<Gated> {
         const Tensor dbg = gradient(bg.defined() && ctx->needs_input_grad(3), bg, {n}, m > 0);
         const Tensor dbu = gradient(bu.defined() && ctx->needs_input_grad(bg.defined() ? 4 : 3), bu, {n}, m > 0);
         if (m > 0) {
+            const Operands o({x, wg, wu}, saved[6]);
             const Tensor d = whole_rows(dh);
             const size_t size = api.workspace_bytes(m, (int)n, (int)k, 1);
             const Tensor ws = bytes(size, x);
-            check(api.gated_bwd(d.data_ptr(), d.stride(0), x.data_ptr(), x.stride(0), wg.data_ptr(), wg.stride(0), wu.data_ptr(), wu.stride(0),
-                                address(saved[5]), address(dx), k, address(dwg), address(dwu), address(dbg), address(dbu), is_fp32(bg) || is_fp32(bu),
+            check(api.gated_bwd(d.data_ptr(), d.stride(0), o.p[0], o.ld[0], o.p[1], o.ld[1], o.p[2], o.ld[2], address(saved[5]), address(dx), k, address(dwg), address(dwu), address(dbg), address(dbu), is_fp32(bg) || is_fp32(bu),
                                 ws.data_ptr(), size, m, (int)n, (int)k, (int)act, dtype_of(x), stream()),
                   "pai_gated_bwd");
         }
@@ -245,7 +281,8 @@ Tensor linear(Tensor x, Tensor w, const std::optional<Tensor> &b_, int64_t act, 
     }
     if (recording({x2, w, b, r})) return shaped(Linear::apply(x2, w, maybe(b), maybe(r), act), x);
     const c10::cuda::CUDAGuard guard(x.device());
-    return shaped(forward(operand(x2), operand(w), Tensor(), b, Tensor(), r, (int)act, nullptr), x);
+    const Tensor xr = whole_rows(x2), wr = whole_rows(w);
+    return shaped(forward(Operands({xr, wr}), xr, wr.size(0), false, b, Tensor(), r, (int)act, nullptr), x);
 }
 
 Tensor gated_linear(Tensor x, Tensor wg, Tensor wu, const std::optional<Tensor> &bg_, const std::optional<Tensor> &bu_, int64_t act) {
@@ -259,8 +296,8 @@ Tensor gated_linear(Tensor x, Tensor wg, Tensor wu, const std::optional<Tensor> 
     const Tensor x2 = flat(x);
     if (recording({x2, wg, wu, bg, bu})) return shaped(Gated::apply(x2, wg, wu, maybe(bg), maybe(bu), act), x);
     const c10::cuda::CUDAGuard guard(x.device());
-    const Tensor a = operand(wg);
-    return shaped(forward(operand(x2), a, wu.is_same(wg) ? a : operand(wu), bg, bu, Tensor(), (int)act, nullptr), x);
+    const Tensor xr = whole_rows(x2), wgr = whole_rows(wg), wur = whole_rows(wu);
+    return shaped(forward(Operands({xr, wgr, wur}), xr, wgr.size(0), true, bg, bu, Tensor(), (int)act, nullptr), x);
 }
 
 }  // namespace
