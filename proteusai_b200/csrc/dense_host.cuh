@@ -155,13 +155,13 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
     const long long ctas = f_tiles * t_tiles * d.groups * splits;
     if (t_tiles * splits > 0x7fffffffll) return (int)PAI_ERR_BAD_SHAPE;
     const int stage = (d.dual ? 2 : 1) * DT_FT * 128 + tn * 128, kb_cta = (p.kb_total + splits - 1) / splits;
-    const int red = splits > 1 ? tn * DT_FT * 4 * (d.dual ? 2 : 1) : 0;  // partial rows sent here
+    const int tile = tn * DT_FT * 4 * (d.dual ? 2 : 1), red = splits > 1 ? tile : 0;  // an fp32 tile; partial rows sent here
     int stages = ((ctas > sms ? 108 : 208) * 1024 - red) / stage;
     stages = stages > DT_MAX_STAGES ? DT_MAX_STAGES : stages;
     stages = stages > kb_cta ? kb_cta : stages;
     p.stages = stages = stages < 1 ? 1 : stages;
     // (the stages also hold the CTA's own partial tile)
-    const int smem = (stages * stage > red ? stages * stage : red) + red + 1024;
+    const int smem = (stages * stage > tile ? stages * stage : tile) + red + 1024;
     const dim3 grid((unsigned)(t_tiles * splits), (unsigned)f_tiles, d.groups);
     CUtensorMap m[4];
     for (int i = 0; i < 2; ++i) {

@@ -1,9 +1,8 @@
 // dense_tile_kernel: out[t, f] = epilogue( sum_r A[f, r] B[t, r] ) on the tensor cores, one output tile of 128 f x tn t per CTA, the
 // reduction split over a cluster where there are too few tiles to fill the GPU.
 //
-// The contiguous axis of the output (f) is the M axis of the MMA, so an accumulator lane is an output column: the 32 lanes of a warp store
-// 64 contiguous bytes of a row, a bias is one register per thread, and a single token costs an MMA of N = 16 rather than 128 rows of
-// which one is wanted.  The same kernel runs every product of the two operators:
+// The contiguous axis of the output (f) is the M axis of the MMA: a few tokens cost an MMA of N = 16 rather than 128 rows of which a few are
+// wanted.  The same kernel runs every product of the two operators:
 //     forward   f = output feature, t = token,           r = input feature:   A = W        (K-major),  B = x  (K-major)
 //     dx        f = input feature,  t = token,           r = output feature:  A = W        (MN-major), B = dz (K-major)
 //     dW        f = input feature,  t = output feature,  r = token:           A = x        (MN-major), B = dz (MN-major)
@@ -69,89 +68,75 @@ __device__ __forceinline__ float load_bias(const void *b, int i, int fp32, int h
     return fp32 ? reinterpret_cast<const float *>(b)[i] : from_bits16(reinterpret_cast<const unsigned short *>(b)[i], half);
 }
 
-// One value of the output from its accumulator(s): column f (bias in b0, b1), row t.
-template <bool DUAL, int ACT>
-__device__ __forceinline__ float dense_finish(const DenseTileParams &p, float v0, float v1, float b0, float b1, int f, int t, int col_blocks) {
-    v0 += b0;
-    if (DUAL) v1 += b1;
-    if (p.save0) {
-        const size_t at = saved_index_f32(t, f, col_blocks);
-        p.save0[at] = v0;
-        if (DUAL) p.save1[at] = v1;
-    }
-    float dummy = 0.f;
-    act_pair<ACT>(v0, dummy);
-    return DUAL ? v0 * v1 : v0;
-}
-
-template <bool DUAL, int ACT, int HALF>
-__device__ __forceinline__ void dense_epilogue(const DenseTileParams &p, uint32_t tmem, float *red, int f, float b0, float b1, int t0,
-                                               int group, int rank) {
-    const int tid = threadIdx.x, warp = tid >> 5;
+// Rows [0, n) of `src` (row r at src + r DT_FT, DUAL: the second accumulator `second` floats behind; `splits` partial tiles `part` floats apart,
+// added in order) are rows first + r of the output.  A warp takes a row at a time, a lane four columns from f: these calls are short chains of
+// instructions on few warps, and a column per thread made this the longest part of a small product.
+template <bool DUAL, int HALF>
+__device__ __forceinline__ void dense_finish(const DenseTileParams &p, const float *src, int splits, int part, int second, int n, int first, int f,
+                                             const float (&b0)[4], const float (&b1)[4], int group) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (f >= p.F) return;
     unsigned short *out = reinterpret_cast<unsigned short *>(group ? p.out1 : p.out0);
-    const int col_blocks = (p.F + 31) >> 5;
-    if (p.splits == 1) {
-        const int q = warp & 3;
-        const bool live = f < p.F;
-        for (int c = (warp >> 2) * 16; c < p.tn; c += 32) {
-            if (t0 + c >= p.T) break;  // (warp-uniform)
-            uint32_t v[16], u[16];
-            tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
-            if (DUAL) tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + p.tn + c, u);
-            float r[16];
-            const int nt = p.T - t0 - c;
-            if (p.residual) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) r[j] = (live && j < nt) ? from_bits16(p.residual[(long long)(t0 + c + j) * p.ld_res + f], HALF) : 0.f;
+    const int col_blocks = (p.F + 31) >> 5, nf = p.F - f;
+    const bool vec_out = nf >= 4 && (p.ld_out & 3) == 0 && ((uintptr_t)out & 7) == 0;
+    const bool vec_res = nf >= 4 && (p.ld_res & 3) == 0 && ((uintptr_t)p.residual & 7) == 0;
+#pragma unroll 1
+    for (int r = warp; r < n; r += DT_THREADS / 32) {
+        const long long t = first + r;
+        unsigned short res[4] = {0, 0, 0, 0};
+        if (p.residual) {
+            const unsigned short *at = p.residual + t * p.ld_res + f;
+            if (vec_res) {
+                const uint2 w = *reinterpret_cast<const uint2 *>(at);
+                res[0] = (unsigned short)w.x, res[1] = (unsigned short)(w.x >> 16), res[2] = (unsigned short)w.y, res[3] = (unsigned short)(w.y >> 16);
             } else {
 #pragma unroll
-                for (int j = 0; j < 16; ++j) r[j] = 0.f;
+                for (int i = 0; i < 4; ++i)
+                    if (i < nf) res[i] = at[i];
             }
-            tmem_wait_ld();
-            if (live) {
+        }
+        float v[4], u[4];
 #pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    if (j < nt) {
-                        const int t = t0 + c + j;
-                        const float y = dense_finish<DUAL, ACT>(p, __uint_as_float(v[j]), DUAL ? __uint_as_float(u[j]) : 0.f, b0, b1, f, t, col_blocks);
-                        out[(long long)t * p.ld_out + f] = to_bits16(y + r[j], HALF);
-                    }
+        for (int i = 0; i < 4; ++i) v[i] = b0[i], u[i] = b1[i];
+        const float *at = src + r * DT_FT + lane * 4;
+        float4 x = *reinterpret_cast<const float4 *>(at), y = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (DUAL) y = *reinterpret_cast<const float4 *>(at + second);
+        for (int s = 1; s < splits; ++s) {
+            at += part;
+            const float4 a = *reinterpret_cast<const float4 *>(at);
+            x.x += a.x, x.y += a.y, x.z += a.z, x.w += a.w;
+            if (DUAL) {
+                const float4 b = *reinterpret_cast<const float4 *>(at + second);
+                y.x += b.x, y.y += b.y, y.z += b.z, y.w += b.w;
             }
-            __syncwarp();
         }
-        return;
-    }
-    // the ranks' partial rows [rank][accumulator][row][128 f]: this CTA's rows [rank, rank + 1) tn / splits of the tile
-    const int fl = tid & 127;
-    if (f >= p.F) return;
-    const int rows = p.tn >> p.split_log, acc = DUAL ? 2 : 1, first = t0 + rank * rows, n = p.T - first < rows ? p.T - first : rows;
-    constexpr int U = 4;
-#pragma unroll 1
-    for (int j0 = tid >> 7; j0 < n; j0 += 2 * U) {
-        float v0[U], v1[U], r[U];
-#pragma unroll
-        for (int k = 0; k < U; ++k) {
-            const int j = j0 + 2 * k;
-            v0[k] = v1[k] = 0.f;
-            r[k] = j < n && p.residual ? from_bits16(p.residual[(long long)(first + j) * p.ld_res + f], HALF) : 0.f;
+        v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+        if (DUAL) u[0] += y.x, u[1] += y.y, u[2] += y.z, u[3] += y.w;
+        if (p.save0) {  // (the buffer's blocks reach past F)
+            const size_t to = saved_index_f32(t, f, col_blocks);
+            *reinterpret_cast<float4 *>(p.save0 + to) = make_float4(v[0], v[1], v[2], v[3]);
+            if (DUAL) *reinterpret_cast<float4 *>(p.save1 + to) = make_float4(u[0], u[1], u[2], u[3]);
         }
-#pragma unroll 1
-        for (int i = 0; i < p.splits; ++i) {
-            const float *src = red + (i * acc * rows + j0) * DT_FT + fl;
-#pragma unroll
-            for (int k = 0; k < U; ++k)
-                if (j0 + 2 * k < n) {
-                    v0[k] += src[2 * k * DT_FT];
-                    if (DUAL) v1[k] += src[(rows + 2 * k) * DT_FT];
-                }
+        switch (p.act) {
+            case ACT_GELU: act_pair<ACT_GELU>(v[0], v[1]), act_pair<ACT_GELU>(v[2], v[3]); break;
+            case ACT_SILU: act_pair<ACT_SILU>(v[0], v[1]), act_pair<ACT_SILU>(v[2], v[3]); break;
+            case ACT_RELU: act_pair<ACT_RELU>(v[0], v[1]), act_pair<ACT_RELU>(v[2], v[3]); break;
+            case ACT_SIGMOID: act_pair<ACT_SIGMOID>(v[0], v[1]), act_pair<ACT_SIGMOID>(v[2], v[3]); break;
+            default: break;
         }
 #pragma unroll
-        for (int k = 0; k < U; ++k)
-            if (j0 + 2 * k < n) {
-                const int t = first + j0 + 2 * k;
-                const float y = dense_finish<DUAL, ACT>(p, v0[k], v1[k], b0, b1, f, t, col_blocks);
-                out[(long long)t * p.ld_out + f] = to_bits16(y + r[k], HALF);
-            }
+        for (int i = 0; i < 4; ++i) {
+            if (DUAL) v[i] *= u[i];
+            if (p.residual) v[i] += from_bits16(res[i], HALF);
+        }
+        unsigned short *o = out + t * p.ld_out + f;
+        if (vec_out) {
+            *reinterpret_cast<uint2 *>(o) = make_uint2(pack_bits16(v[0], v[1], HALF), pack_bits16(v[2], v[3], HALF));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (i < nf) o[i] = to_bits16(v[i], HALF);
+        }
     }
 }
 
@@ -178,7 +163,7 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
     uint32_t cols = 32;
     while (cols < (uint32_t)p.tn * ACC) cols <<= 1;
 
-    const int f = f0 + (int)(threadIdx.x & 127);  // this thread's output column: its lane of the accumulator
+    const int f = f0 + lane * 4;  // this thread's four output columns in the epilogue
     // (the loops of warps 0 and 1 are run by the whole warp, one elected thread issues: control flow and descriptors stay warp-uniform)
     const bool leader = warp < 2 && elect_one();
     auto load = [&](int kb, int slot) {
@@ -200,7 +185,8 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
             tma_load_2d(b, mb, r, t0, &bar_full[slot]);
         }
     };
-    const int ahead = k1 - k0 < p.stages ? k1 - k0 : p.stages;  // loads that need no free slot: under way before the rest is set up
+    const int fresh = k1 - k0 < p.stages ? k1 - k0 : p.stages;  // loads that need no free slot; the first two are under way before the rest is set up
+    const int ahead = fresh < 2 ? fresh : 2;
     if (warp == 0) {
         if (leader) {
             for (int i = 0; i < p.stages; ++i) {
@@ -227,9 +213,12 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
     const uint32_t tmem = tmem_base;
 
     if (warp == 0) {
-        int slot = ahead == p.stages ? 0 : ahead;
-        uint32_t phase = ahead == p.stages ? 1 : 0;
-        for (int kb = k0 + ahead; kb < k1; ++kb) {
+        if (leader)
+            for (int i = ahead; i < fresh; ++i) load(k0 + i, i);
+        __syncwarp();
+        int slot = fresh == p.stages ? 0 : fresh;
+        uint32_t phase = fresh == p.stages ? 1 : 0;
+        for (int kb = k0 + fresh; kb < k1; ++kb) {
             if (!mbar_wait_abortable(&bar_free[slot], phase ^ 1, &abort_flag)) break;
             if (leader) load(kb, slot);
             __syncwarp();
@@ -265,68 +254,59 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
         if (ok && leader) umma_commit(&bar_done);
     }
     __syncwarp();
-    const float b0 = p.bias0 && f < p.F ? load_bias(p.bias0, f, p.bias_fp32, HALF) : 0.f;  // (on its way while the products run)
-    const float b1 = DUAL && p.bias1 && f < p.F ? load_bias(p.bias1, f, p.bias_fp32, HALF) : 0.f;
+    float b0[4], b1[4];  // (on their way while the products run)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        b0[i] = p.bias0 && f + i < p.F ? load_bias(p.bias0, f + i, p.bias_fp32, HALF) : 0.f;
+        b1[i] = DUAL && p.bias1 && f + i < p.F ? load_bias(p.bias1, f + i, p.bias_fp32, HALF) : 0.f;
+    }
     bool ok = mbar_wait_abortable(&bar_done, 0, &abort_flag);
     tc_fence_after();
-    if (p.splits > 1) {
-        float *mine = reinterpret_cast<float *>(base);  // the stages have been read: this CTA's partial tile [accumulator][tn][128]
-        if (ok) {
-            const int q = warp & 3;
-            for (int c = (warp >> 2) * 16; c < p.tn * ACC; c += 32) {
-                const int tc = DUAL && c >= p.tn ? c - p.tn : c;
-                if (t0 + tc >= p.T) continue;  // (warp-uniform)
-                uint32_t v[16];
-                tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
-                tmem_wait_ld();
+    float *mine = reinterpret_cast<float *>(base);  // over the stages, which have been read: this CTA's tile [accumulator][tn][128]
+    if (ok) {
+        const int q = warp & 3;
+        for (int c = (warp >> 2) * 16; c < p.tn * ACC; c += 32) {
+            const int tc = DUAL && c >= p.tn ? c - p.tn : c;
+            if (t0 + tc >= p.T) continue;  // (warp-uniform)
+            uint32_t v[16];
+            tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + c, v);
+            tmem_wait_ld();
+            float *to = mine + c * DT_FT + q * 32 + lane;
 #pragma unroll
-                for (int j = 0; j < 16; ++j) mine[(c + j) * DT_FT + q * 32 + lane] = __uint_as_float(v[j]);
-            }
+            for (int j = 0; j < 16; ++j) to[j * DT_FT] = __uint_as_float(v[j]);
         }
-        fence_proxy_async();
-        tc_fence_before();
-        __syncthreads();
-        if (warp == 2) {
-            tc_fence_after();
-            tmem_relinquish();
-            tmem_dealloc(tmem, cols);
-        }
-        __syncwarp();
+    }
+    if (p.splits > 1) fence_proxy_async();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_relinquish();
+        tmem_dealloc(tmem, cols);
+    }
+    __syncwarp();
+    const int first = t0 + rank * rows, left = p.T - first, n = left < rows ? left : rows;  // rows that are this CTA's to finish
+    if (p.splits > 1) {
         cluster_wait();  // every CTA of the cluster has its barriers: it can be sent to
         if (warp == 0 && lane < p.splits && ok) {
-            const int left = p.T - t0 - lane * rows, n = left < 0 ? 0 : left < rows ? left : rows;  // rows that rank `lane` finishes
+            const int left_to = p.T - t0 - lane * rows, to = left_to < 0 ? 0 : left_to < rows ? left_to : rows;  // rows that rank `lane` finishes
             const uint32_t bar = map_to_rank(smem_u32(&bar_red), lane);
 #pragma unroll
             for (int a = 0; a < ACC; ++a)
-                if (n > 0)
+                if (to > 0)
                     bulk_s2s(map_to_rank(smem_u32(red + (rank * ACC + a) * rows * DT_FT), lane), mine + (a * p.tn + lane * rows) * DT_FT,
-                             (uint32_t)n * DT_FT * 4, bar);
+                             (uint32_t)to * DT_FT * 4, bar);
         }
         __syncwarp();
         ok = mbar_wait_abortable(&bar_red, 0, &abort_flag) && ok;
         cluster_arrive();
     }
     if (ok) {
-        switch (p.act) {
-            case ACT_GELU: dense_epilogue<DUAL, ACT_GELU, HALF>(p, tmem, red, f, b0, b1, t0, group, rank); break;
-            case ACT_SILU: dense_epilogue<DUAL, ACT_SILU, HALF>(p, tmem, red, f, b0, b1, t0, group, rank); break;
-            case ACT_RELU: dense_epilogue<DUAL, ACT_RELU, HALF>(p, tmem, red, f, b0, b1, t0, group, rank); break;
-            case ACT_SIGMOID: dense_epilogue<DUAL, ACT_SIGMOID, HALF>(p, tmem, red, f, b0, b1, t0, group, rank); break;
-            default: dense_epilogue<DUAL, ACT_NONE, HALF>(p, tmem, red, f, b0, b1, t0, group, rank);
-        }
+        if (p.splits > 1) dense_finish<DUAL, HALF>(p, red, p.splits, ACC * rows * DT_FT, rows * DT_FT, n, first, f, b0, b1, group);
+        else dense_finish<DUAL, HALF>(p, mine, 1, 0, p.tn * DT_FT, n, first, f, b0, b1, group);
     }
     __syncwarp();
-    if (p.splits > 1) {
-        cluster_wait();  // what this CTA sent has been received
-    } else {
-        tc_fence_before();
-        __syncthreads();
-        if (warp == 2) {
-            tc_fence_after();
-            tmem_relinquish();
-            tmem_dealloc(tmem, cols);
-        }
-    }
+    if (p.splits > 1) cluster_wait();  // what this CTA sent has been received
 }
 
 }  // namespace pai
