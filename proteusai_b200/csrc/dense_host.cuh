@@ -51,14 +51,16 @@ struct DenseTune {
 };
 static DenseTune g_dense_tune;
 
-// The kernel and its shape are the ones with the lowest estimated time, in cycles.
+// The kernel and its shape are the ones with the lowest estimated time, in microseconds: models with coefficients fitted to 1143 measurements of all
+// shapes at 19 sizes from 16 x 512 x 2048 to 16384 x 512 x 2048 (both fit within 7 % r.m.s.; the choice is within 10 % of the best shape on
+// nearly all of them).
 struct DenseChoice {
     int pair, width, splits;   // width: rows t of a tile (tile kernel), accumulator columns (pair kernel)
     double cost;
 };
 
-// Tile kernel: a CTA's 64-wide reduction block costs the larger of its MMAs (2 tn cycles per accumulator) and its loads (the SM takes about
-// 48 bytes a cycle from L2); CTAs beyond one per SM queue up; a split adds the exchange of partial tiles.
+// Tile kernel: start and end; per 64-wide reduction block the instructions of its loads and MMAs; per row of the tile the epilogue, shared by
+// the CTAs of a split reduction but with its exchange.  Clusters of 4 and 8 leave SMs of a GPC unused.
 static DenseChoice dense_tile_choose(const DenseProduct &d, int sms) {
     const long long kb = (d.R + DT_BK - 1) / DT_BK * d.segs;
     const int acc = d.dual ? 2 : 1, least = d.b_mn ? 64 : 16;
@@ -70,21 +72,21 @@ static DenseChoice dense_tile_choose(const DenseProduct &d, int sms) {
         for (int splits = 1; splits <= 8 && splits <= kb; splits *= 2) {
             if (g_dense_tune.kernel == 1 && g_dense_tune.splits && splits != g_dense_tune.splits) continue;
             if (splits > 1 && tn * acc > 128) continue;  // (the partial rows' buffer)
-            const double rounds = (double)((tiles * splits + sms - 1) / sms);
-            const double mma = 2.0 * tn * acc, load = (128.0 * acc + tn) * 128.0 / 48.0;
-            const double work = (double)((kb + splits - 1) / splits) * (mma > load ? mma : load);
-            const double epi = (splits > 1 ? 1500.0 + tn * acc * 8.0 + (double)tn / splits * 20.0 * acc : tn * 12.0 * acc);
-            const double t = rounds * (work + epi) + 2500.0;
+            const long long room = splits == 8 ? sms * 3 / 4 : splits == 4 ? sms * 8 / 9 : sms;
+            const double rounds = (double)((tiles * splits + room - 1) / room), blocks = (double)((kb + splits - 1) / splits), w = tn * acc;
+            const double cta = blocks * (0.317 + 0.00024 * w + (d.dual ? 0.037 : 0.0)) + 0.0236 * w / splits + (splits > 1 ? 1.0 + 0.0274 * w : 0.0);
+            const double t = 3.6 + (rounds > 1 ? 1.1 * rounds : 1.0) * cta;
             if (t < best.cost) best = {0, tn, splits, t};
         }
     }
     return best;
 }
 
-// Pair kernel: 2 bn cycles per reduction block, one tile in flight per pair of SMs, 5000 cycles to start and to finish the last tile.  A split
-// reduction writes and reads fp32 tiles (about 2000 bytes a cycle for the whole GPU) and adds a launch.
+// Pair kernel: start and end; per tile the products of its reduction and what of the epilogue they do not cover; a split reduction writes and
+// reads fp32 tiles and adds a launch.
 static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_split) {
     const long long kb = (d.R + DT_BK - 1) / DT_BK * d.segs;
+    const double out = 1e-6 * (double)d.F * (double)d.T * d.groups;
     DenseChoice best = {1, 256, 1, 1e300};
     for (int bn = d.dual ? 256 : 128; bn <= 256; bn *= 2) {
         if (g_dense_tune.kernel == 2 && g_dense_tune.width && bn != g_dense_tune.width) continue;
@@ -92,11 +94,9 @@ static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_sp
         const long long tiles = (d.F + fw - 1) / fw * ((d.T + 255) / 256) * d.groups;
         for (int splits = 1; splits <= (may_split ? 16 : 1) && splits * 4 <= (kb > 4 ? kb : 4); ++splits) {
             if (g_dense_tune.kernel == 2 && g_dense_tune.splits && may_split && splits != g_dense_tune.splits) continue;
-            const double rounds = (double)((tiles * splits + sms / 2 - 1) / (sms / 2));
-            const double block = bn == 256 ? 560.0 : 400.0, epi = bn * 14.0;
-            const double work = (double)((kb + splits - 1) / splits) * block;
-            double t = rounds * (work > epi ? work : epi) + epi + 5000.0;
-            if (splits > 1) t += 5000.0 + 2.0 * splits * d.groups * (double)d.F * d.T * 4.0 / 2000.0;
+            const double rounds = (double)((tiles * splits + sms / 2 - 1) / (sms / 2)), blocks = (double)((kb + splits - 1) / splits);
+            const double tile = bn == 256 ? 0.29 * blocks + 0.84 : 0.237 * blocks + 0.3;
+            const double t = 5.6 + rounds * tile + 0.16 * out + (splits > 1 ? 5.6 + 1.0 * splits * out : 0.0);
             if (t < best.cost) best = {1, bn, splits, t};
         }
     }
