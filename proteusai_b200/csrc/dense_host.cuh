@@ -180,18 +180,33 @@ static int make_operand_map(CUtensorMap *m, const DenseOperand &o, int mn, long 
     return mn ? make_map_16(m, o.p, rows, R, o.ld, 64, half) : make_map_16(m, o.p, R, rows, o.ld, box, half);
 }
 
-template <int MODE, int HALF>
+template <int MODE, int HALF, int FLAGS>
 static int dense_pair_launch_as(const CUtensorMap (&m)[6], const DensePairParams &p, int ctas, cudaStream_t st) {
     static bool attr_done[64];
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel<MODE, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DensePairSmem));
+        cudaError_t e = cudaFuncSetAttribute(dense_pair_kernel<MODE, HALF, FLAGS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(DensePairSmem));
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    dense_pair_kernel<MODE, HALF><<<ctas, DP_THREADS, sizeof(DensePairSmem), st>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
+    dense_pair_kernel<MODE, HALF, FLAGS><<<ctas, DP_THREADS, sizeof(DensePairSmem), st>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
     return (int)cudaPeekAtLastError();
+}
+
+template <int HALF>
+static int dense_pair_launch_half(const CUtensorMap (&m)[6], const DensePairParams &p, int dual, int flags, int ctas, cudaStream_t st) {
+    if (dual) {
+        if (flags == DP_ANY) return dense_pair_launch_as<DP_GATED, HALF, DP_ANY>(m, p, ctas, st);
+        return flags ? dense_pair_launch_as<DP_GATED, HALF, DP_SAVE>(m, p, ctas, st) : dense_pair_launch_as<DP_GATED, HALF, 0>(m, p, ctas, st);
+    }
+    switch (flags) {
+        case 0: return dense_pair_launch_as<DP_LINEAR, HALF, 0>(m, p, ctas, st);
+        case DP_RESIDUAL: return dense_pair_launch_as<DP_LINEAR, HALF, DP_RESIDUAL>(m, p, ctas, st);
+        case DP_SAVE: return dense_pair_launch_as<DP_LINEAR, HALF, DP_SAVE>(m, p, ctas, st);
+        case DP_RESIDUAL | DP_SAVE: return dense_pair_launch_as<DP_LINEAR, HALF, DP_RESIDUAL | DP_SAVE>(m, p, ctas, st);
+        default: return dense_pair_launch_as<DP_LINEAR, HALF, DP_ANY>(m, p, ctas, st);
+    }
 }
 
 // (in the roles of DenseProduct the pair kernel's rows are t, its columns f: its A is `b`, its B is `a`)
@@ -240,14 +255,15 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
         if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half, 32)) return e;
     const int ctas = 2 * (int)(items < sms / 2 ? items : sms / 2);
     if (partial) {
-        if (int e = dense_pair_launch_as<DP_PARTIAL, 0>(m, p, ctas, st)) return e;
+        if (int e = dense_pair_launch_as<DP_PARTIAL, 0, 0>(m, p, ctas, st)) return e;
         const size_t blocks = saved_blocks(d.T, (int)d.F);
         dense_reduce_kernel<<<dim3((unsigned)((blocks + 7) / 8), d.groups), 256, 0, st>>>(d.part, (unsigned short *)d.out[0], (unsigned short *)d.out[1],
                                                                                         p.T, p.F, d.ld_out, d.groups, c.splits, d.half);
         return (int)cudaPeekAtLastError();
     }
-    if (d.half) return d.dual ? dense_pair_launch_as<DP_GATED, 1>(m, p, ctas, st) : dense_pair_launch_as<DP_LINEAR, 1>(m, p, ctas, st);
-    return d.dual ? dense_pair_launch_as<DP_GATED, 0>(m, p, ctas, st) : dense_pair_launch_as<DP_LINEAR, 0>(m, p, ctas, st);
+    const int any = !p.tma_out || (d.residual && !p.tma_res) ? DP_ANY : 0;
+    const int flags = any ? any : (d.residual ? DP_RESIDUAL : 0) | (d.save[0] ? DP_SAVE : 0);
+    return d.half ? dense_pair_launch_half<1>(m, p, d.dual, flags, ctas, st) : dense_pair_launch_half<0>(m, p, d.dual, flags, ctas, st);
 }
 
 static int dense_launch(const DenseProduct &d, int sms, cudaStream_t st) {
