@@ -257,7 +257,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     if (partial) {
         if (int e = dense_pair_launch_as<DP_PARTIAL, 0, 0>(m, p, ctas, st)) return e;
         const size_t blocks = saved_blocks(d.T, (int)d.F);
-        dense_reduce_kernel<<<dim3((unsigned)((blocks + 7) / 8), d.groups), 256, 0, st>>>(d.part, (unsigned short *)d.out[0], (unsigned short *)d.out[1],
+        dense_reduce_kernel<<<dim3((unsigned)blocks, d.groups), 256, 0, st>>>(d.part, (unsigned short *)d.out[0], (unsigned short *)d.out[1],
                                                                                         p.T, p.F, d.ld_out, d.groups, c.splits, d.half);
         return (int)cudaPeekAtLastError();
     }

@@ -231,7 +231,10 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
             }
     };
     if (has_bias) fetch_biases(t);
-    if (res_tma && lane == 0) fetch_residual(t, 0, 0);
+    if (res_tma && lane == 0) {
+        fetch_residual(t, 0, 0);
+        if (panels > 1) fetch_residual(t, 1, 1);
+    }
     uint32_t res_phase = 0;  // bit b: phase of res_full[b]
     int used = 0;            // panels so far
     for (int n = 0; t.valid(); ++n) {
@@ -280,7 +283,7 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
                     __syncwarp();
                 }
                 if (has_res && !res_tma && live) {  // any alignment: a row at a time, a column per lane
-#pragma unroll 4
+#pragma unroll 16
                     for (int r = 0; r < 32; ++r) {
                         const unsigned short v =
                             row0 + r < p.T && col + lane < p.F ? p.residual[(long long)(row0 + r) * p.ld_res + col + lane] : (unsigned short)0;
@@ -347,7 +350,7 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
                             *reinterpret_cast<const unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2);
                 __syncwarp();
             }
-            if (res_tma && lane == 0) {  // the next panel's residual into the other buffer, once the store before this one has read it
+            if (res_tma && lane == 0 && (used > 1 || panels == 1)) {  // the next panel's residual, once the store before this one has read its buffer
                 bulk_wait_read<1>();
                 fence_proxy_async();
                 if (i + 1 < panels) fetch_residual(t, i + 1, b ^ 1);
@@ -500,36 +503,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
     }
 }
 
-// out[group][t, f] = sum over splits of the partial tiles, in order of the splits; one warp per block of 32 x 32
+// out[group][t, f] = sum over splits of the partial tiles, in order of the splits; a CTA per block of 32 x 32, a warp per four rows of it
 __global__ void __launch_bounds__(256) dense_reduce_kernel(const float *__restrict__ part, unsigned short *out0, unsigned short *out1, int T, int F,
                                                            long long ld_out, int groups, int splits, int half) {
     const int lane = threadIdx.x & 31, col_blocks = (F + 31) >> 5;
-    const size_t matrix = saved_bytes_f32(T, F) / 4, blocks = matrix / 1024;
-    const size_t b = (size_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (b >= blocks) return;
-    const int group = blockIdx.y;
+    const size_t matrix = saved_bytes_f32(T, F) / 4, b = blockIdx.x;
+    const int group = blockIdx.y, r = (threadIdx.x >> 5) * 4 + (lane >> 3);
     unsigned short *out = group ? out1 : out0;
-    const int t0 = (int)(b / col_blocks) * 32, f = (int)(b % col_blocks) * 32 + (lane & 7) * 4;
-    const bool vec = (ld_out & 3) == 0 && ((uintptr_t)out & 7) == 0;
+    const int t = (int)(b / col_blocks) * 32 + r, f = (int)(b % col_blocks) * 32 + (lane & 7) * 4;
+    const float *src = part + group * matrix + b * 1024 + (lane & 7) * 128 + r * 4;
+    float4 s = *reinterpret_cast<const float4 *>(src);
+#pragma unroll 4
+    for (int i = 1; i < splits; ++i) {
+        const float4 v = *reinterpret_cast<const float4 *>(src + (size_t)i * groups * matrix);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    if (t >= T) return;
+    unsigned short *o = out + (long long)t * ld_out + f;
+    if ((ld_out & 3) == 0 && ((uintptr_t)out & 7) == 0 && f + 4 <= F) {
+        *reinterpret_cast<uint2 *>(o) = make_uint2(pack_bits16(s.x, s.y, half), pack_bits16(s.z, s.w, half));
+    } else {
+        const float e[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-        const int r = g * 4 + (lane >> 3);
-        float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < splits; ++i) {
-            const float4 v = *reinterpret_cast<const float4 *>(part + (size_t)(i * groups + group) * matrix + b * 1024 + (lane & 7) * 128 + r * 4);
-            s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
-        }
-        if (t0 + r < T) {
-            unsigned short *o = out + (long long)(t0 + r) * ld_out + f;
-            if (vec && f + 4 <= F) {
-                *reinterpret_cast<uint2 *>(o) = make_uint2(pack_bits16(s.x, s.y, half), pack_bits16(s.z, s.w, half));
-            } else {
-                const float e[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (f + i < F) o[i] = to_bits16(e[i], half);
-            }
-        }
+        for (int i = 0; i < 4; ++i)
+            if (f + i < F) o[i] = to_bits16(e[i], half);
     }
 }
 
