@@ -12,7 +12,9 @@ are then unused), ``"beta_abs"`` (the reference tree's ``S + beta Rn |S|`` with 
 with the reference's own kernel expects), or ``None`` for the default of ``geometric_attn``.
 
 ``Encoder`` is the reference's post-norm block (``old/old_scripts/encoder.py:8-41``): ``LN(x + drop(attn))``
-then ``LN(x + drop(ffn))``, each one fused kernel in bf16 inference.  The reference's ``forward`` passes ``coords_beta`` positionally into a
+then ``LN(x + drop(ffn))``, each one fused kernel in bf16 inference.  ``ffn`` (an addition) chooses the feed-forward block: ``"mlp"`` (the
+reference's, on PyTorch's products), ``"fused"`` (the same block and parameters, its products with their epilogues as one kernel each) or
+``"gated"`` (``GatedMLP``).  The reference's ``forward`` passes ``coords_beta`` positionally into a
 ``GeoAttention.forward`` that has no such parameter (a TypeError there); here it is accepted and unused.
 """
 import torch
@@ -22,7 +24,7 @@ import torch.nn.functional as F
 from proteusai_b200.utils.model_utils.attn import geometric_attn as _ga
 from proteusai_b200.utils.model_utils.attn.geometric_attn import geometric_attn, spreads_known_positive
 from proteusai_b200.utils.model_utils.base_modules import fused_ops
-from proteusai_b200.utils.model_utils.base_modules.base_modules import MLP
+from proteusai_b200.utils.model_utils.base_modules.base_modules import MLP, GatedMLP
 from proteusai_b200.utils.model_utils.wf_embedding.wf_embedding import WaveFunctionEmbedding
 
 
@@ -128,27 +130,47 @@ class GeoAttention(nn.Module):
 
 
 class Encoder(nn.Module):
+    ffn_kind = "mlp"
 
     def __init__(self, d_model=512, heads=8, min_spread=2.0, min_rbf=0.001, d_hidden=2048, hidden_layers=0,
-                 dropout=0.10, learn_spreads=True, logit_form=None):
+                 dropout=0.10, learn_spreads=True, logit_form=None, ffn="mlp"):
         super().__init__()
+        if ffn not in ("mlp", "fused", "gated"):
+            raise ValueError(f"ffn must be 'mlp', 'fused' or 'gated', not {ffn!r}")
+        if ffn == "gated" and hidden_layers:
+            raise ValueError("a gated feed-forward block has no further hidden layers")
+        self.ffn_kind = ffn
         self.attn = GeoAttention(d_model=d_model, heads=heads, min_spread=min_spread, min_rbf=min_rbf, learn_spreads=learn_spreads,
                                  logit_form=logit_form)
         self.attn_norm = nn.LayerNorm(d_model)
-        self.ffn = MLP(d_in=d_model, d_out=d_model, d_hidden=d_hidden, hidden_layers=hidden_layers, dropout=dropout)
+        if ffn == "gated":
+            self.ffn = GatedMLP(d_in=d_model, d_out=d_model, d_hidden=d_hidden, dropout=dropout)
+        else:
+            self.ffn = MLP(d_in=d_model, d_out=d_model, d_hidden=d_hidden, hidden_layers=hidden_layers, dropout=dropout, fused=ffn == "fused")
         self.ffn_norm = nn.LayerNorm(d_model)
         self.dropout = nn.Dropout(dropout)
 
+    def _drop_off(self):
+        return not self.training or self.dropout.p == 0.0
+
     def _add_norm(self, x, y, norm):
         """``norm(x + dropout(y))``: one fused pass for bf16 inference, the PyTorch operators otherwise."""
-        drop_off = not self.training or self.dropout.p == 0.0
-        if drop_off and x.shape[-1] % 8 == 0 and x.shape[-1] <= 4096 and fused_ops.usable(x, y, norm.weight, norm.bias):
+        if self._drop_off() and x.shape[-1] % 8 == 0 and x.shape[-1] <= 4096 and fused_ops.usable(x, y, norm.weight, norm.bias):
             return fused_ops.add_layernorm(x, y, norm.weight, norm.bias, norm.eps)
         return norm(x + self.dropout(y))
 
+    def _ffn_norm(self, x):
+        """``norm(x + dropout(ffn(x)))``, the sum in the epilogue of the block's last product where nothing stands between."""
+        if self.ffn_kind == "mlp" or not self._drop_off():
+            return self._add_norm(x, self.ffn(x), self.ffn_norm)
+        y, norm = self.ffn(x, residual=x), self.ffn_norm
+        if y.shape[-1] % 8 == 0 and y.shape[-1] <= 4096 and fused_ops.usable(y, norm.weight, norm.bias):
+            return fused_ops.add_layernorm(y, None, norm.weight, norm.bias, norm.eps)
+        return norm(y)
+
     def forward(self, q, k, v, coords, coords_beta=None, mask=None):
         q = self._add_norm(q, self.attn(q, k, v, coords, mask=mask), self.attn_norm)
-        return self._add_norm(q, self.ffn(q), self.ffn_norm)
+        return self._ffn_norm(q)
 
 
 class ProteusEncoderModel(nn.Module):
@@ -157,11 +179,11 @@ class ProteusEncoderModel(nn.Module):
     README, ``README.md:38,48``, from the modules above)."""
 
     def __init__(self, d_model=512, heads=8, layers=4, d_hidden=2048, vocab=33, n_out=20, sigma_lo=3.0, sigma_hi=15.0,
-                 min_wl=3.7, max_wl=20.0, base_wl=20.0):
+                 min_wl=3.7, max_wl=20.0, base_wl=20.0, ffn="mlp"):
         super().__init__()
         self.embed = nn.Embedding(vocab, d_model)
         self.wf_embedding = WaveFunctionEmbedding(d_wf=d_model, min_wl=min_wl, max_wl=max_wl, base_wl=base_wl, anisotropic=False)
-        self.encoders = nn.ModuleList(Encoder(d_model=d_model, heads=heads, d_hidden=d_hidden, dropout=0.0) for _ in range(layers))
+        self.encoders = nn.ModuleList(Encoder(d_model=d_model, heads=heads, d_hidden=d_hidden, dropout=0.0, ffn=ffn) for _ in range(layers))
         self.head = nn.Linear(d_model, n_out)
         # spreads linearly spaced in [sigma_lo, sigma_hi]: spread = min_spread + exp(w)
         sig = torch.linspace(sigma_lo, sigma_hi, heads)

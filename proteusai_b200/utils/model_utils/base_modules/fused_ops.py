@@ -67,6 +67,11 @@ def dense_usable(*tensors):
     return ts[0].dtype in (torch.bfloat16, torch.float16) and all(t.dtype == ts[0].dtype for t in ts)
 
 
+def dense_dtype(x):
+    """The type in which ``linear`` and ``gated_linear`` compute for an ``x`` they take."""
+    return torch.get_autocast_dtype("cuda") if torch.is_autocast_enabled("cuda") else x.dtype
+
+
 def _act_code(what, act):
     code = ACTIVATIONS.get(act, -1)
     if code < 0:
