@@ -241,6 +241,21 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
         const int row0 = row_of(t), a = n & 1;
         DensePairTiles next = t;
         next.next(p);
+        if (has_res && !res_tma) {  // any alignment: a row at a time, a column per lane, both panels (at most two) before the products are done
+            if (lane == 0) bulk_wait_read<0>();
+            __syncwarp();
+            for (int i = 0; i < panels; ++i) {
+                const int col = col_of(t, i) + lane, rows = p.T - row0;
+                uint8_t *panel = sm.panel[ew][(used + i) & 1];
+                const unsigned short *src = p.residual + (long long)row0 * p.ld_res + col;
+                unsigned short w[32];
+#pragma unroll
+                for (int r = 0; r < 32; ++r) w[r] = r < rows && col < p.F ? src[(long long)r * p.ld_res] : (unsigned short)0;
+#pragma unroll
+                for (int r = 0; r < 32; ++r) *reinterpret_cast<unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2) = w[r];
+            }
+            __syncwarp();
+        }
         if (!mbar_wait_abortable(&sm.acc_full[a], (n >> 1) & 1, &sm.abort_flag)) break;
         tc_fence_after();
         const uint32_t acc = tmem + a * 256 + ((uint32_t)(q * 32) << 16) + g * panels * 32;
@@ -273,22 +288,14 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
             const bool first = (c & 31) == 0, last = ((c + STEP) & 31) == 0;
             uint8_t *panel = sm.panel[ew][b];
             if (MODE != DP_PARTIAL && first) {
-                if (res_tma) {
+                if (has_res && !res_tma) {  // (the panel holds the residual already)
+                } else if (res_tma) {
                     if (live) {
                         mbar_wait_abortable(&sm.res_full[ew][b], (res_phase >> b) & 1, &sm.abort_flag);
                         res_phase ^= 1u << b;
                     }
                 } else {
                     if (lane == 0) bulk_wait_read<1>();  // the store before the last one has read this buffer
-                    __syncwarp();
-                }
-                if (has_res && !res_tma && live) {  // any alignment: a row at a time, a column per lane
-#pragma unroll 16
-                    for (int r = 0; r < 32; ++r) {
-                        const unsigned short v =
-                            row0 + r < p.T && col + lane < p.F ? p.residual[(long long)(row0 + r) * p.ld_res + col + lane] : (unsigned short)0;
-                        *reinterpret_cast<unsigned short *>(panel + sw64_offset(r, lane >> 3) + (lane & 7) * 2) = v;
-                    }
                     __syncwarp();
                 }
             }
@@ -343,7 +350,7 @@ __device__ __forceinline__ void dense_pair_epilogue(const DensePairParams &p, De
                 }
             } else if (live) {
                 __syncwarp();
-#pragma unroll 4
+#pragma unroll 8
                 for (int r = 0; r < 32; ++r)
                     if (row0 + r < p.T && col + lane < p.F)
                         p.out0[(long long)(row0 + r) * p.ld_out + col + lane] =
