@@ -52,6 +52,12 @@ __device__ __forceinline__ void sfu_sincos(float x, float &s, float &c) {
     asm("cos.approx.ftz.f32 %0, %1;" : "=f"(c) : "f"(x));
 }
 
+// Programmatic dependent launch.  A kernel launched with it may be brought onto the SMs while the one before it still runs, once that one's CTAs have
+// all called pdl_trigger; pdl_wait returns when it has finished and its writes are visible.  (Without the launch attribute both do nothing.)
+// A kernel that allocates tensor memory triggers after it has: one that came early could otherwise hold the columns that it waits for.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // 2^x on the SFU
 __device__ __forceinline__ float ex2_approx(float x) {
     float y;

@@ -24,6 +24,25 @@ static int make_map_16(CUtensorMap *map, const void *base, long long inner, long
     return r == CUDA_SUCCESS ? 0 : (int)PAI_ERR_UNSUPPORTED;
 }
 
+// Launch as a programmatic dependent of what is on the stream (common.cuh), in clusters of `cluster` CTAs if it is more than 1.
+template <typename... P, typename... A>
+static int dense_launch_kernel(void (*kernel)(P...), dim3 grid, int block, int smem, cudaStream_t st, int cluster, const A &...args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+}
+
 struct DenseOperand {       // a matrix of 16-bit elements
     const void *p;
     long long ld;
@@ -119,18 +138,7 @@ static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(DT_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)p.splits;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, dense_tile_kernel<DUAL, HALF>, m[0], m[1], m[2], m[3], p);
+    return dense_launch_kernel(dense_tile_kernel<DUAL, HALF>, grid, DT_THREADS, smem, st, p.splits, m[0], m[1], m[2], m[3], p);
 }
 
 static uint32_t dense_idesc(int m, int n, const DenseProduct &d, int m_mn, int n_mn) {
@@ -190,8 +198,8 @@ static int dense_pair_launch_as(const CUtensorMap (&m)[6], const DensePairParams
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    dense_pair_kernel<MODE, HALF, FLAGS><<<ctas, DP_THREADS, sizeof(DensePairSmem), st>>>(m[0], m[1], m[2], m[3], m[4], m[5], p);
-    return (int)cudaPeekAtLastError();
+    return dense_launch_kernel(dense_pair_kernel<MODE, HALF, FLAGS>, dim3(ctas), DP_THREADS, (int)sizeof(DensePairSmem), st, 1, m[0], m[1], m[2], m[3],
+                               m[4], m[5], p);
 }
 
 template <int HALF>
@@ -257,9 +265,8 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     if (partial) {
         if (int e = dense_pair_launch_as<DP_PARTIAL, 0, 0>(m, p, ctas, st)) return e;
         const size_t blocks = saved_blocks(d.T, (int)d.F);
-        dense_reduce_kernel<<<dim3((unsigned)blocks, d.groups), 256, 0, st>>>(d.part, (unsigned short *)d.out[0], (unsigned short *)d.out[1],
-                                                                                        p.T, p.F, d.ld_out, d.groups, c.splits, d.half);
-        return (int)cudaPeekAtLastError();
+        return dense_launch_kernel(dense_reduce_kernel, dim3((unsigned)blocks, d.groups), 256, 0, st, 1, d.part, d.out[0], d.out[1], p.T, p.F, d.ld_out,
+                                   d.groups, c.splits, d.half);
     }
     const int any = !p.tma_out || (d.residual && !p.tma_res) ? DP_ANY : 0;
     const int flags = any ? any : (d.residual ? DP_RESIDUAL : 0) | (d.save[0] ? DP_SAVE : 0);
@@ -273,29 +280,28 @@ static int dense_launch(const DenseProduct &d, int sms, cudaStream_t st) {
 
 // ---- up to eight tokens ---------------------------------------------------------------------------------------------
 template <bool DUAL, int ACT, int TT>
-static void dense_vec_as(const DenseVecParams &p, int half, unsigned grid, cudaStream_t st) {
-    if (half) dense_vec_kernel<DUAL, ACT, TT, 1><<<grid, DV_WARPS * 32, 0, st>>>(p);
-    else dense_vec_kernel<DUAL, ACT, TT, 0><<<grid, DV_WARPS * 32, 0, st>>>(p);
+static int dense_vec_as(const DenseVecParams &p, int half, unsigned grid, cudaStream_t st) {
+    return half ? dense_launch_kernel(dense_vec_kernel<DUAL, ACT, TT, 1>, dim3(grid), DV_WARPS * 32, 0, st, 1, p)
+                : dense_launch_kernel(dense_vec_kernel<DUAL, ACT, TT, 0>, dim3(grid), DV_WARPS * 32, 0, st, 1, p);
 }
 template <bool DUAL, int ACT>
-static void dense_vec_tokens(const DenseVecParams &p, int half, unsigned grid, cudaStream_t st) {
-    if (p.T <= 1) dense_vec_as<DUAL, ACT, 1>(p, half, grid, st);
-    else if (p.T <= 2) dense_vec_as<DUAL, ACT, 2>(p, half, grid, st);
-    else if (p.T <= 4) dense_vec_as<DUAL, ACT, 4>(p, half, grid, st);
-    else dense_vec_as<DUAL, ACT, 8>(p, half, grid, st);
+static int dense_vec_tokens(const DenseVecParams &p, int half, unsigned grid, cudaStream_t st) {
+    if (p.T <= 1) return dense_vec_as<DUAL, ACT, 1>(p, half, grid, st);
+    if (p.T <= 2) return dense_vec_as<DUAL, ACT, 2>(p, half, grid, st);
+    if (p.T <= 4) return dense_vec_as<DUAL, ACT, 4>(p, half, grid, st);
+    return dense_vec_as<DUAL, ACT, 8>(p, half, grid, st);
 }
 template <bool DUAL>
 static int dense_vec_act(const DenseVecParams &p, int act, int half, cudaStream_t st) {
     const int per_cta = DV_WARPS * (DUAL ? 1 : 2);
     const unsigned grid = (unsigned)((p.N + per_cta - 1) / per_cta);
     switch (act) {
-        case ACT_GELU: dense_vec_tokens<DUAL, ACT_GELU>(p, half, grid, st); break;
-        case ACT_SILU: dense_vec_tokens<DUAL, ACT_SILU>(p, half, grid, st); break;
-        case ACT_RELU: dense_vec_tokens<DUAL, ACT_RELU>(p, half, grid, st); break;
-        case ACT_SIGMOID: dense_vec_tokens<DUAL, ACT_SIGMOID>(p, half, grid, st); break;
-        default: dense_vec_tokens<DUAL, ACT_NONE>(p, half, grid, st);
+        case ACT_GELU: return dense_vec_tokens<DUAL, ACT_GELU>(p, half, grid, st);
+        case ACT_SILU: return dense_vec_tokens<DUAL, ACT_SILU>(p, half, grid, st);
+        case ACT_RELU: return dense_vec_tokens<DUAL, ACT_RELU>(p, half, grid, st);
+        case ACT_SIGMOID: return dense_vec_tokens<DUAL, ACT_SIGMOID>(p, half, grid, st);
+        default: return dense_vec_tokens<DUAL, ACT_NONE>(p, half, grid, st);
     }
-    return (int)cudaPeekAtLastError();
 }
 static bool dense_uses_vec(long long T) { return T <= DV_MAX_TOKENS && (g_dense_tune.kernel == 0 || g_dense_tune.kernel == 3); }
 static int dense_vec_launch(const DenseProduct &d, cudaStream_t st) {
@@ -376,13 +382,13 @@ static size_t dense_bwd_workspace(long long M, int N, int K, int mats, int sms) 
 }
 
 template <bool DUAL, int ACT>
-static void dense_bwd_elem_as(const DenseBwdElemParams &p, int half, bool f32, dim3 grid, cudaStream_t st) {
-    if (half) dense_bwd_elem_kernel<DUAL, ACT, 1, true><<<grid, 256, 0, st>>>(p);
-    else if (f32) dense_bwd_elem_kernel<DUAL, ACT, 0, true><<<grid, 256, 0, st>>>(p);
-    else dense_bwd_elem_kernel<DUAL, ACT, 0, false><<<grid, 256, 0, st>>>(p);
+static int dense_bwd_elem_as(const DenseBwdElemParams &p, int half, bool f32, dim3 grid, cudaStream_t st) {
+    if (half) return dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 1, true>, grid, 256, 0, st, 1, p);
+    return f32 ? dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 0, true>, grid, 256, 0, st, 1, p)
+               : dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 0, false>, grid, 256, 0, st, 1, p);
 }
 template <bool DUAL>
-static void dense_bwd_elem_act(const DenseBwdElemParams &p, int act, int half, bool f32, dim3 grid, cudaStream_t st) {
+static int dense_bwd_elem_act(const DenseBwdElemParams &p, int act, int half, bool f32, dim3 grid, cudaStream_t st) {
     switch (act) {
         case ACT_GELU: return dense_bwd_elem_as<DUAL, ACT_GELU>(p, half, f32, grid, st);
         case ACT_SILU: return dense_bwd_elem_as<DUAL, ACT_SILU>(p, half, f32, grid, st);
@@ -393,9 +399,7 @@ static void dense_bwd_elem_act(const DenseBwdElemParams &p, int act, int half, b
 }
 static int dense_bwd_elem_launch(const DenseBwdElemParams &p, bool gated, int act, int half, bool f32, unsigned strips, cudaStream_t st) {
     const dim3 grid((p.N + 255) / 256, strips);
-    if (gated) dense_bwd_elem_act<true>(p, act, half, f32, grid, st);
-    else dense_bwd_elem_act<false>(p, act, half, f32, grid, st);
-    return (int)cudaPeekAtLastError();
+    return gated ? dense_bwd_elem_act<true>(p, act, half, f32, grid, st) : dense_bwd_elem_act<false>(p, act, half, f32, grid, st);
 }
 
 static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const DenseOperand (&w)[2], const void *saved, void *dx, long long lddx,
@@ -436,8 +440,7 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
         const float *first = db[0] ? p.part0 : p.part1;
         void *out = db[0] ? db[0] : db[1];
         const dim3 grid((N + 31) / 32, db[0] && db[1] ? 2 : 1);
-        dense_colsum_kernel<<<grid, 256, 0, st>>>(first, p.part1, out, db[1], N, (int)strips, half, bias_fp32);
-        if (int e = (int)cudaPeekAtLastError()) return e;
+        if (int e = dense_launch_kernel(dense_colsum_kernel, grid, 256, 0, st, 1, first, p.part1, out, db[1], N, (int)strips, half, bias_fp32)) return e;
     }
     if (dx) {
         DenseProduct d = {};
@@ -466,8 +469,7 @@ static int dense_copy_rows(const DenseCopyParams &p, int count, int sms, cudaStr
     if (most == 0) return 0;
     long long blocks = (most + 255) / 256;
     if (blocks > (long long)sms * 16) blocks = (long long)sms * 16;
-    dense_copy_rows_kernel<<<dim3((unsigned)blocks, count), 256, 0, st>>>(p);
-    return (int)cudaPeekAtLastError();
+    return dense_launch_kernel(dense_copy_rows_kernel, dim3((unsigned)blocks, count), 256, 0, st, 1, p);
 }
 
 }  // namespace pai

@@ -182,6 +182,8 @@ struct DenseBwdElemParams {
 
 template <bool DUAL, int ACT, int HALF, bool F32>
 __global__ void __launch_bounds__(256) dense_bwd_elem_kernel(const __grid_constant__ DenseBwdElemParams p) {
+    pdl_trigger();
+    pdl_wait();
     constexpr bool PLAIN = !DUAL && ACT == ACT_NONE;  // sums of dy alone
     constexpr int U = 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -275,6 +277,8 @@ __global__ void __launch_bounds__(256) dense_bwd_elem_kernel(const __grid_consta
 // out[c] = sum over strips of part[s, c], in order of s
 __global__ void __launch_bounds__(256) dense_colsum_kernel(const float *__restrict__ part0, const float *__restrict__ part1, void *out0, void *out1,
                                                            int N, int strips, int half, int out_fp32) {
+    pdl_trigger();
+    pdl_wait();
     const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
     const float *part = blockIdx.y ? part1 : part0;
     void *out = blockIdx.y ? out1 : out0;
@@ -300,6 +304,8 @@ struct DenseCopyParams {
     int cols[DENSE_MAX_COPIES];
 };
 __global__ void __launch_bounds__(256) dense_copy_rows_kernel(const __grid_constant__ DenseCopyParams p) {
+    pdl_trigger();
+    pdl_wait();
     const int m = blockIdx.y, cols = p.cols[m], words = (cols + 7) >> 3;
     const long long n = p.rows[m] * words, stride = (long long)gridDim.x * 256;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += stride) {

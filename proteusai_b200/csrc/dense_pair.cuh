@@ -409,6 +409,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
     cluster_wait();  // both CTAs' barriers are ready
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
+    pdl_trigger();
+    pdl_wait();
 
     // (The loops of warps 0 and 1 are run by the whole warp, one elected thread issuing: control flow and descriptors stay warp-uniform, which keeps
     // the instructions between two products few.  Run by one thread alone they took 620 cycles per reduction block, and 1200 beside a busy
@@ -513,6 +515,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
 // out[group][t, f] = sum over splits of the partial tiles, in order of the splits; a CTA per block of 32 x 32, a warp per four rows of it
 __global__ void __launch_bounds__(256) dense_reduce_kernel(const float *__restrict__ part, unsigned short *out0, unsigned short *out1, int T, int F,
                                                            long long ld_out, int groups, int splits, int half) {
+    pdl_trigger();
+    pdl_wait();
     const int lane = threadIdx.x & 31, col_blocks = (F + 31) >> 5;
     const size_t matrix = saved_bytes_f32(T, F) / 4, b = blockIdx.x;
     const int group = blockIdx.y, r = (threadIdx.x >> 5) * 4 + (lane >> 3);

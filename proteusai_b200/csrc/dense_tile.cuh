@@ -201,9 +201,14 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
                 const int left = p.T - t0 - rank * rows;
                 mbar_expect_tx(&bar_red, (uint32_t)(p.splits * ACC * (left < 0 ? 0 : left < rows ? left : rows) * DT_FT * 4));
             }
-            for (int i = 0; i < ahead; ++i) load(k0 + i, i);
         }
         __syncwarp();
+        pdl_wait();
+        if (leader)
+            for (int i = 0; i < ahead; ++i) load(k0 + i, i);
+        __syncwarp();
+    } else {
+        pdl_wait();
     }
     if (p.splits > 1) cluster_arrive();  // (this CTA's barriers are ready)
     if (warp == 2) tmem_alloc(&tmem_base, cols);
@@ -211,6 +216,7 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base;
+    pdl_trigger();
 
     if (warp == 0) {
         if (leader)

@@ -24,6 +24,8 @@ struct DenseVecParams {
 
 template <bool DUAL, int ACT, int TT, int HALF>
 __global__ void __launch_bounds__(DV_WARPS * 32) dense_vec_kernel(const __grid_constant__ DenseVecParams p) {
+    pdl_trigger();
+    pdl_wait();
     constexpr int U = TT <= 2 ? 4 : 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int f = ((int)blockIdx.x * DV_WARPS + warp) * (DUAL ? 1 : 2);
