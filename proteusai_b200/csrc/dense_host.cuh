@@ -104,7 +104,7 @@ static DenseChoice dense_tile_choose(const DenseProduct &d, int sms) {
 // Pair kernel: start and end; per tile the products of its reduction and what of the epilogue they do not cover; a split reduction writes and
 // reads fp32 tiles and adds a launch.
 static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_split) {
-    const long long kb = (d.R + DT_BK - 1) / DT_BK * d.segs;
+    const long long kb = (d.R + DP_BK - 1) / DP_BK * d.segs;
     const double out = 1e-6 * (double)d.F * (double)d.T * d.groups;
     DenseChoice best = {1, 256, 1, 1e300};
     for (int bn = d.dual ? 256 : 128; bn <= 256; bn *= 2) {
@@ -134,7 +134,7 @@ static int dense_tile_launch_as(const CUtensorMap (&m)[4], const DenseTileParams
     int dev = 0;
     cudaGetDevice(&dev);
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        cudaError_t e = cudaFuncSetAttribute(dense_tile_kernel<DUAL, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+        cudaError_t e = cudaFuncSetAttribute(dense_tile_kernel<DUAL, HALF>, cudaFuncAttributeMaxDynamicSharedMemorySize, 224 * 1024);
         if (e != cudaSuccess) return (int)e;
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
@@ -157,14 +157,15 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
     const long long f_tiles = (d.F + DT_FT - 1) / DT_FT, t_tiles = (d.T + tn - 1) / tn;  // (f_tiles <= 2^13: widths are limited)
     p.splits = splits, p.split_log = splits == 8 ? 3 : splits == 4 ? 2 : splits == 2 ? 1 : 0, p.tn = tn;
     p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
+    p.tail = d.R % DT_BK > 0 && d.R % DT_BK <= 64;
     p.a_mn = d.a_mn, p.b_mn = d.b_mn;
     p.act = d.act, p.bias_fp32 = d.bias_fp32;
     p.idesc = dense_idesc(128, tn, d, d.a_mn, d.b_mn);
     const long long ctas = f_tiles * t_tiles * d.groups * splits;
     if (t_tiles * splits > 0x7fffffffll) return (int)PAI_ERR_BAD_SHAPE;
-    const int stage = (d.dual ? 2 : 1) * DT_FT * 128 + tn * 128, kb_cta = (p.kb_total + splits - 1) / splits;
+    const int stage = (d.dual ? 2 : 1) * DT_FT * 256 + tn * 256, kb_cta = (p.kb_total + splits - 1) / splits;
     const int tile = tn * DT_FT * 4 * (d.dual ? 2 : 1), red = splits > 1 ? tile : 0;  // an fp32 tile; partial rows sent here
-    int stages = ((ctas > sms ? 108 : 208) * 1024 - red) / stage;
+    int stages = ((ctas > sms && 2 * stage + red <= 108 * 1024 ? 108 : 216) * 1024 - red) / stage;  // two CTAs per SM if two stages each fit
     stages = stages > DT_MAX_STAGES ? DT_MAX_STAGES : stages;
     stages = stages > kb_cta ? kb_cta : stages;
     p.stages = stages = stages < 1 ? 1 : stages;
@@ -175,9 +176,9 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
     for (int i = 0; i < 2; ++i) {
         const DenseOperand &a = d.a[i].p ? d.a[i] : d.a[0], &b = d.b[i].p ? d.b[i] : d.b[0];
         if (i == 1 && !d.a[1].p) m[1] = m[0];
-        else if (int e = d.a_mn ? make_map_16(&m[i], a.p, d.F, d.R, a.ld, 64, d.half) : make_map_16(&m[i], a.p, d.R, d.F, a.ld, DT_FT, d.half)) return e;
+        else if (int e = d.a_mn ? make_map_16(&m[i], a.p, d.F, d.R, a.ld, DT_BK, d.half) : make_map_16(&m[i], a.p, d.R, d.F, a.ld, DT_FT, d.half)) return e;
         if (i == 1 && !d.b[1].p) m[3] = m[2];
-        else if (int e = d.b_mn ? make_map_16(&m[2 + i], b.p, d.T, d.R, b.ld, 64, d.half) : make_map_16(&m[2 + i], b.p, d.R, d.T, b.ld, tn, d.half)) return e;
+        else if (int e = d.b_mn ? make_map_16(&m[2 + i], b.p, d.T, d.R, b.ld, DT_BK, d.half) : make_map_16(&m[2 + i], b.p, d.R, d.T, b.ld, tn, d.half)) return e;
     }
     if (d.half) return d.dual ? dense_tile_launch_as<true, 1>(m, p, grid, smem, st) : dense_tile_launch_as<false, 1>(m, p, grid, smem, st);
     return d.dual ? dense_tile_launch_as<true, 0>(m, p, grid, smem, st) : dense_tile_launch_as<false, 0>(m, p, grid, smem, st);
@@ -241,7 +242,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     p.ld_out = d.ld_out, p.ld_res = d.ld_res;
     p.T = (int)d.T, p.F = (int)d.F, p.bn = c.width;
     p.t_tiles = (int)((d.T + 255) / 256), p.f_tiles = (int)((d.F + fw - 1) / fw), p.groups = d.groups, p.splits = c.splits;
-    p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
+    p.kb_seg = (int)((d.R + DP_BK - 1) / DP_BK), p.kb_total = p.kb_seg * d.segs;
     p.a_mn = d.b_mn, p.b_mn = d.a_mn, p.act = d.act;
     p.idesc = dense_idesc(256, c.width, d, d.b_mn, d.a_mn);
     const long long items = (long long)p.t_tiles * p.f_tiles * p.groups * p.splits;

@@ -19,6 +19,7 @@
 
 namespace pai {
 
+constexpr int DP_BK = 64;  // reduction block: 128 bytes, one swizzle row
 constexpr int DP_STAGES = 5;
 constexpr int DP_STAGE_BYTES = 32768;  // A 128 x 128 bytes, B up to 128 x 128 bytes
 constexpr int DP_EPI_WARPS = 16;
@@ -435,7 +436,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
                     if (rank == 0) mbar_expect_tx(&sm.full[slot], bytes);
                     const uint32_t bar = full0 + slot * 8;
                     const bool second = kb >= p.kb_seg;
-                    const int r = (second ? kb - p.kb_seg : kb) * DT_BK;
+                    const int r = (second ? kb - p.kb_seg : kb) * DP_BK;
                     const CUtensorMap *mA = (second || group) ? &ma1 : &ma0;
                     const CUtensorMap *mB = (second || (MODE == DP_GATED && rank)) ? &mb1 : &mb0;
                     if (p.a_mn) {

@@ -9,7 +9,7 @@
 // Gated forward: two A operands (Wg, Wu) against one B into two accumulators (DUAL).  Gated dx: two pairs of operands in sequence into one
 // accumulator (kb_seg).  Gated dW: two output groups (the second with its own B and output).
 //
-// Split reduction: the CTAs of a cluster each take a run of the 64-wide reduction blocks and send their partial rows to the CTA that finishes
+// Split reduction: the CTAs of a cluster each take a run of the reduction blocks and send their partial rows to the CTA that finishes
 // them (tn / splits rows each) by bulk copies into its shared memory; that CTA adds the partials of all ranks in rank order: one launch, no
 // workspace, no atomics, the same bits every time.  The cluster barriers around the copies are arrived at long before they are waited for.
 //
@@ -22,7 +22,7 @@ namespace pai {
 
 constexpr int DT_THREADS = 256;
 constexpr int DT_FT = 128;        // output columns (MMA rows) per tile
-constexpr int DT_BK = 64;         // reduction block: 128 bytes, one swizzle row
+constexpr int DT_BK = 128;        // reduction block: two swizzle rows of 64.  (With 64 the wait, commit and loop around four MMAs cost as much as they.)
 constexpr int DT_MAX_STAGES = 8;
 
 struct DenseTileParams {
@@ -33,7 +33,8 @@ struct DenseTileParams {
     long long ld_out, ld_res;
     int F, T;
     int splits, split_log, tn, stages;  // splits = 1 << split_log; grid: x = t tile * splits + rank, y = f tile, z = group
-    int kb_seg, kb_total;           // 64-wide reduction blocks of the first operand pair, of both
+    int kb_seg, kb_total;           // reduction blocks of the first operand pair, of both
+    int tail;                       // the last block of a pair has 64 columns at most
     int a_mn, b_mn;                 // operands stored with the reduction as their slow axis
     int act, bias_fp32;
     uint32_t idesc;
@@ -156,7 +157,8 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
     const int k0 = (p.kb_total * rank) >> p.split_log, k1 = (p.kb_total * (rank + 1)) >> p.split_log;
     const int rows = p.tn >> p.split_log;  // rows of the tile that this CTA finishes
     constexpr int ACC = DUAL ? 2 : 1;
-    const uint32_t a_bytes = ACC * DT_FT * 128, b_bytes = (uint32_t)p.tn * 128;
+    // a stage: A (DUAL: both), B, each two K-major tiles of 64 columns or 64-wide panels of 128 steps of the reduction
+    const uint32_t a_bytes = ACC * DT_FT * 256, b_bytes = (uint32_t)p.tn * 256, b_half = (uint32_t)p.tn * 128;
     const uint32_t stage_bytes = a_bytes + b_bytes;
     const uint32_t tile_bytes = (uint32_t)p.tn * ACC * DT_FT * 4;  // a whole partial tile, sent (over the stages) and received (behind them)
     float *red = reinterpret_cast<float *>(base + ((uint32_t)p.stages * stage_bytes > tile_bytes ? (uint32_t)p.stages * stage_bytes : tile_bytes));
@@ -174,15 +176,20 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
         const CUtensorMap *ma = second ? &ma1 : &ma0, *mb = (second || group) ? &mb1 : &mb0;
         if (p.a_mn) {
             tma_load_2d(a, ma, f0, r, &bar_full[slot]);
-            tma_load_2d(a + 8192, ma, f0 + 64, r, &bar_full[slot]);
+            tma_load_2d(a + 16384, ma, f0 + 64, r, &bar_full[slot]);
         } else {
             tma_load_2d(a, ma, r, f0, &bar_full[slot]);
-            if (DUAL) tma_load_2d(a + 16384, &ma1, r, f0, &bar_full[slot]);
+            tma_load_2d(a + 16384, ma, r + 64, f0, &bar_full[slot]);
+            if (DUAL) {
+                tma_load_2d(a + 32768, &ma1, r, f0, &bar_full[slot]);
+                tma_load_2d(a + 49152, &ma1, r + 64, f0, &bar_full[slot]);
+            }
         }
         if (p.b_mn) {
-            for (int i = 0; i < p.tn; i += 64) tma_load_2d(b + i * 128, mb, t0 + i, r, &bar_full[slot]);
+            for (int i = 0; i < p.tn; i += 64) tma_load_2d(b + i * 256, mb, t0 + i, r, &bar_full[slot]);
         } else {
             tma_load_2d(b, mb, r, t0, &bar_full[slot]);
+            tma_load_2d(b + b_half, mb, r + 64, t0, &bar_full[slot]);
         }
     };
     const int fresh = k1 - k0 < p.stages ? k1 - k0 : p.stages;  // loads that need no free slot; the first two are under way before the rest is set up
@@ -231,11 +238,12 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
             if (++slot == p.stages) slot = 0, phase ^= 1;
         }
     } else if (warp == 1) {
-        // K-major: rows of 128 bytes, 8-row groups 1024 apart, 16 elements of the reduction 32 bytes on.
-        // MN-major: 64-wide panels 8192 apart, 8 steps of the reduction 1024 apart, 16 of them 2048 on.
+        // K-major: rows of 128 bytes, 8-row groups 1024 apart, 16 elements of the reduction 32 bytes on, the next 64 in the next tile.
+        // MN-major: 64-wide panels 16384 apart, 8 steps of the reduction 1024 apart, 16 of them 2048 on.
         const uint32_t a_step = (p.a_mn ? 2048 : 32) >> 4, b_step = (p.b_mn ? 2048 : 32) >> 4;
-        const uint64_t ad0 = umma_desc_sw128(smem_u32(base), p.a_mn ? 8192 : 16, 1024);
-        const uint64_t bd0 = umma_desc_sw128(smem_u32(base) + a_bytes, p.b_mn ? 8192 : 16, 1024);
+        const uint32_t a_next = (p.a_mn ? 8192 : 16384) >> 4, b_next = (p.b_mn ? 8192 : b_half) >> 4;
+        const uint64_t ad0 = umma_desc_sw128(smem_u32(base), p.a_mn ? 16384 : 16, 1024);
+        const uint64_t bd0 = umma_desc_sw128(smem_u32(base) + a_bytes, p.b_mn ? 16384 : 16, 1024);
         int slot = 0;
         uint32_t phase = 0;
         bool ok = true;
@@ -247,11 +255,17 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
             tc_fence_after();
             if (leader) {
                 const uint64_t ad = ad0 + (uint64_t)(slot * (stage_bytes >> 4)), bd = bd0 + (uint64_t)(slot * (stage_bytes >> 4));
+                const bool half = p.tail && (kb + 1 == p.kb_seg || kb + 1 == p.kb_total);  // (its second 64 columns are zeros)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    umma_ss(tmem, ad + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
-                    if (DUAL) umma_ss(tmem + p.tn, ad + (16384 >> 4) + k * a_step, bd + k * b_step, p.idesc, kb > k0 || k > 0);
-                }
+                for (int h = 0; h < 2; ++h)
+                    if (h == 0 || !half) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint64_t ak = ad + h * a_next + k * a_step, bk = bd + h * b_next + k * b_step;
+                            umma_ss(tmem, ak, bk, p.idesc, kb > k0 || h > 0 || k > 0);
+                            if (DUAL) umma_ss(tmem + p.tn, ak + (32768 >> 4), bk, p.idesc, kb > k0 || h > 0 || k > 0);
+                        }
+                    }
                 umma_commit(&bar_free[slot]);
             }
             __syncwarp();
