@@ -70,15 +70,15 @@ struct DenseTune {
 };
 static DenseTune g_dense_tune;
 
-// The kernel and its shape are the ones with the lowest estimated time, in microseconds: models with coefficients fitted to 1143 measurements of all
-// shapes at 19 sizes from 16 x 512 x 2048 to 16384 x 512 x 2048 (both fit within 7 % r.m.s.; the choice is within 10 % of the best shape on
-// nearly all of them).
+// The kernel and its shape are the ones with the lowest estimated time, in microseconds: models with coefficients fitted to 699 measurements of all
+// shapes at 19 sizes from 16 x 512 x 2048 to 16384 x 512 x 2048, one product after another on a stream (r.m.s. 9 and 7 %; the choice is within
+// 9 % of the best shape on all 76 products).
 struct DenseChoice {
     int pair, width, splits;   // width: rows t of a tile (tile kernel), accumulator columns (pair kernel)
     double cost;
 };
 
-// Tile kernel: start and end; per 64-wide reduction block the instructions of its loads and MMAs; per row of the tile the epilogue, shared by
+// Tile kernel: start and end; per reduction block the instructions of its loads and MMAs; per row of the tile the epilogue, shared by
 // the CTAs of a split reduction but with its exchange.  Clusters of 4 and 8 leave SMs of a GPC unused.
 static DenseChoice dense_tile_choose(const DenseProduct &d, int sms) {
     const long long kb = (d.R + DT_BK - 1) / DT_BK * d.segs;
@@ -93,8 +93,8 @@ static DenseChoice dense_tile_choose(const DenseProduct &d, int sms) {
             if (splits > 1 && tn * acc > 128) continue;  // (the partial rows' buffer)
             const long long room = splits == 8 ? sms * 3 / 4 : splits == 4 ? sms * 8 / 9 : sms;
             const double rounds = (double)((tiles * splits + room - 1) / room), blocks = (double)((kb + splits - 1) / splits), w = tn * acc;
-            const double cta = blocks * (0.317 + 0.00024 * w + (d.dual ? 0.037 : 0.0)) + 0.0236 * w / splits + (splits > 1 ? 1.0 + 0.0274 * w : 0.0);
-            const double t = 3.6 + (rounds > 1 ? 1.1 * rounds : 1.0) * cta;
+            const double cta = 0.81 + blocks * (0.426 + 0.00083 * w + (d.dual ? 0.156 : 0.0)) + 0.0243 * w / splits + (splits > 1 ? 0.49 + 0.036 * w : 0.0);
+            const double t = 1.8 + (rounds > 1 ? 1.08 * rounds : 1.0) * cta;
             if (t < best.cost) best = {0, tn, splits, t};
         }
     }
@@ -111,11 +111,11 @@ static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_sp
         if (g_dense_tune.kernel == 2 && g_dense_tune.width && bn != g_dense_tune.width) continue;
         const int fw = d.dual ? bn / 2 : bn;
         const long long tiles = (d.F + fw - 1) / fw * ((d.T + 255) / 256) * d.groups;
-        for (int splits = 1; splits <= (may_split ? 16 : 1) && splits * 4 <= (kb > 4 ? kb : 4); ++splits) {
+        for (int splits = 1; splits <= (may_split ? 8 : 1) && splits * 4 <= (kb > 4 ? kb : 4); ++splits) {
             if (g_dense_tune.kernel == 2 && g_dense_tune.splits && may_split && splits != g_dense_tune.splits) continue;
             const double rounds = (double)((tiles * splits + sms / 2 - 1) / (sms / 2)), blocks = (double)((kb + splits - 1) / splits);
-            const double tile = bn == 256 ? 0.29 * blocks + 0.84 : 0.237 * blocks + 0.3;
-            const double t = 5.6 + rounds * tile + 0.16 * out + (splits > 1 ? 5.6 + 1.0 * splits * out : 0.0);
+            const double tile = bn == 256 ? 0.29 * blocks + 0.46 : 0.237 * blocks;
+            const double t = 3.85 + rounds * tile + 0.287 * out + (splits > 1 ? 1.65 + 1.54 * splits * out : 0.0);
             if (t < best.cost) best = {1, bn, splits, t};
         }
     }
