@@ -61,6 +61,7 @@ struct DenseProduct {
     long long ld_res;
     void *save[2];
     int act, half;
+    DenseColsum colsum;        // bias gradients that the product's kernel finishes
     float *part;               // workspace of a split reduction in the pair kernel (dense_pair_choose), or NULL: no split
 };
 
@@ -158,6 +159,7 @@ static int dense_tile_launch(const DenseProduct &d, const DenseChoice &c, int sm
     p.splits = splits, p.split_log = splits == 8 ? 3 : splits == 4 ? 2 : splits == 2 ? 1 : 0, p.tn = tn;
     p.kb_seg = (int)((d.R + DT_BK - 1) / DT_BK), p.kb_total = p.kb_seg * d.segs;
     p.tail = d.R % DT_BK > 0 && d.R % DT_BK <= 64;
+    p.colsum = d.colsum;
     p.a_mn = d.a_mn, p.b_mn = d.b_mn;
     p.act = d.act, p.bias_fp32 = d.bias_fp32;
     p.idesc = dense_idesc(128, tn, d, d.a_mn, d.b_mn);
@@ -226,6 +228,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
             e.groups = 1;
             e.b[0] = d.b[g], e.b[1] = {nullptr, 0};
             e.out[0] = d.out[g], e.out[1] = nullptr;
+            if (g > 0) e.colsum = {};
             if (int r = dense_pair_launch(e, c, sms, st)) return r;
         }
         return 0;
@@ -239,6 +242,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     p.save_f32 = d.half;
     p.save_exps = (long long)saved_blocks(d.T, (int)d.F) * 2048;
     p.part = d.part;
+    p.colsum = d.colsum;
     p.ld_out = d.ld_out, p.ld_res = d.ld_res;
     p.T = (int)d.T, p.F = (int)d.F, p.bn = c.width;
     p.t_tiles = (int)((d.T + 255) / 256), p.f_tiles = (int)((d.F + fw - 1) / fw), p.groups = d.groups, p.splits = c.splits;
@@ -264,7 +268,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
         if (int e = make_map_16(&m[5], d.residual, d.F, d.T, d.ld_res, 32, d.half, 32)) return e;
     const int ctas = 2 * (int)(items < sms / 2 ? items : sms / 2);
     if (partial) {
-        if (int e = dense_pair_launch_as<DP_PARTIAL, 0, 0>(m, p, ctas, st)) return e;
+        if (int e = d.half ? dense_pair_launch_as<DP_PARTIAL, 1, 0>(m, p, ctas, st) : dense_pair_launch_as<DP_PARTIAL, 0, 0>(m, p, ctas, st)) return e;
         const size_t blocks = saved_blocks(d.T, (int)d.F);
         return dense_launch_kernel(dense_reduce_kernel, dim3((unsigned)blocks, d.groups), 256, 0, st, 1, d.part, d.out[0], d.out[1], p.T, p.F, d.ld_out,
                                    d.groups, c.splits, d.half);
@@ -436,12 +440,14 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
     if ((elementwise && products) || p.part0) {
         if (int e = dense_bwd_elem_launch(p, gated, act, half, f32, (unsigned)strips, st)) return e;
     }
+    DenseColsum colsum = {};
     if (p.part0) {
-        // (one of two bias gradients alone: its own sums go into the grid's first row)
-        const float *first = db[0] ? p.part0 : p.part1;
-        void *out = db[0] ? db[0] : db[1];
-        const dim3 grid((N + 31) / 32, db[0] && db[1] ? 2 : 1);
-        if (int e = dense_launch_kernel(dense_colsum_kernel, grid, 256, 0, st, 1, first, p.part1, out, db[1], N, (int)strips, half, bias_fp32)) return e;
+        colsum = {{db[0] ? p.part0 : nullptr, db[1] ? p.part1 : nullptr}, {db[0], db[1]}, N, (int)strips, bias_fp32};
+        if (!products) {
+            const dim3 grid((N + 31) / 32);
+            return half ? dense_launch_kernel(dense_colsum_kernel<1>, grid, 32, 0, st, 1, colsum)
+                        : dense_launch_kernel(dense_colsum_kernel<0>, grid, 32, 0, st, 1, colsum);
+        }
     }
     if (dx) {
         DenseProduct d = {};
@@ -450,6 +456,8 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
         d.segs = mats, d.groups = 1;
         d.F = K, d.T = M, d.R = N;
         d.out[0] = dx, d.ld_out = lddx, d.half = half;
+        d.colsum = colsum;
+        colsum = {};
         if (int e = dense_launch(d, sms, st)) return e;
     }
     if (dw[0] || dw[1]) {
@@ -458,6 +466,7 @@ static int dense_backward(const DenseOperand &dy, const DenseOperand &x, const D
         d.b[0] = dw[0] ? dz[0] : dz[1], d.out[0] = dw[0] ? dw[0] : dw[1];
         if (d.groups == 2) d.b[1] = dz[1], d.out[1] = dw[1];
         d.ld_out = K, d.half = half;
+        d.colsum = colsum;
         d.part = (float *)(ws + mats * (dense_d_bytes(M, N) + dense_part_bytes(M, N)));
         if (int e = dense_launch(d, sms, st)) return e;
     }

@@ -166,8 +166,7 @@ struct Saved8 {
 // ---- elementwise half of the backward pass ------------------------------------------------------------------------
 // One warp covers 8 rows x 32 columns a step (4 lanes x 8 columns per row), a CTA 8 rows x 256 columns; it walks down a strip of
 // `strip` rows, two steps' loads in flight, and keeps the column sums of what it writes in registers (the bias gradients), joined over the
-// eight row lanes by shuffles and written as one partial row per strip; dense_colsum_kernel adds the strips in order, so the sums are
-// reproducible.  HBM-bound: gated in bf16 reads dh, g, u and writes dg, du, 10 bytes per element.
+// eight row lanes by shuffles and written as one partial row per strip; dense_colsum adds the strips.  HBM-bound: gated in bf16 reads dh, g, u and writes dg, du, 10 bytes per element.
 struct DenseBwdElemParams {
     const unsigned short *dy;
     long long ld_dy;
@@ -274,25 +273,44 @@ __global__ void __launch_bounds__(256) dense_bwd_elem_kernel(const __grid_consta
     }
 }
 
-// out[c] = sum over strips of part[s, c], in order of s
-__global__ void __launch_bounds__(256) dense_colsum_kernel(const float *__restrict__ part0, const float *__restrict__ part1, void *out0, void *out1,
-                                                           int N, int strips, int half, int out_fp32) {
+// ---- bias gradients: out[c] = sum over strips of part[s, c] -------------------------------------------------------
+// The product that follows the elementwise pass does it with a warp that has nothing else to do (a launch of its own would cost a small backward
+// pass several microseconds of host time); dense_colsum_kernel where no product follows.  Lane: a column; sixteen partial sums over the strips
+// s = i mod 16, added in order of i: the same bits wherever it runs.
+struct DenseColsum {
+    const float *part[2];  // NULL: none
+    void *out[2];
+    int N, strips, fp32;
+};
+
+template <int HALF>
+__device__ __forceinline__ void dense_colsum(const DenseColsum &c, int warp, int warps) {
+    const int lane = threadIdx.x & 31;
+    for (int m = 0; m < 2; ++m) {
+        if (!c.part[m]) continue;
+        for (int col = warp * 32 + lane; col < c.N; col += warps * 32) {
+            constexpr int U = 16;
+            float s[U];
+#pragma unroll
+            for (int k = 0; k < U; ++k) s[k] = 0.f;
+            for (int i = 0; i < c.strips; i += U)
+#pragma unroll
+                for (int k = 0; k < U; ++k)
+                    if (i + k < c.strips) s[k] += c.part[m][(size_t)(i + k) * c.N + col];
+            float sum = s[0];
+#pragma unroll
+            for (int k = 1; k < U; ++k) sum += s[k];
+            if (c.fp32) reinterpret_cast<float *>(c.out[m])[col] = sum;
+            else reinterpret_cast<unsigned short *>(c.out[m])[col] = to_bits16(sum, HALF);
+        }
+    }
+}
+
+template <int HALF>
+__global__ void __launch_bounds__(32) dense_colsum_kernel(const __grid_constant__ DenseColsum c) {
     pdl_trigger();
     pdl_wait();
-    const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
-    const float *part = blockIdx.y ? part1 : part0;
-    void *out = blockIdx.y ? out1 : out0;
-    __shared__ float sm[8][32];
-    float s = 0.f;
-    if (c < N)
-        for (int i = w; i < strips; i += 8) s += part[(size_t)i * N + c];
-    sm[w][threadIdx.x & 31] = s;
-    __syncthreads();
-    if (w == 0 && c < N) {
-        for (int i = 1; i < 8; ++i) s += sm[i][threadIdx.x];
-        if (out_fp32) reinterpret_cast<float *>(out)[c] = s;
-        else reinterpret_cast<unsigned short *>(out)[c] = to_bits16(s, half);
-    }
+    dense_colsum<HALF>(c, (int)blockIdx.x, (int)gridDim.x);
 }
 
 // dst[r, 0 .. cols) = src[r, 0 .. cols) for rows of any alignment (TMA wants 16-byte aligned ones), up to three matrices in a launch

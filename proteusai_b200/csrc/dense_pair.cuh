@@ -13,7 +13,8 @@
 //     dW       t = output feature,  f = input feature,  r = token:          A = dz (MN-major), B = x (MN-major); the long reduction split
 //              over pairs that leave fp32 tiles in the workspace, added in order by dense_reduce_kernel
 //
-// Warps: 0 TMA loads, 1 MMAs (first CTA of the pair), 2 tensor memory, 4..11 epilogue (two per quarter of the lanes, half the columns each).
+// Warps: 0 TMA loads, 1 MMAs (first CTA of the pair), 2 tensor memory, 3 what is left of the bias gradients, 4..19 epilogue (four per quarter of
+// the lanes, a quarter of the columns each; eight with twice the columns and registers took 178 us for 148 with GELU at 65536 x 512 x 2048).
 #pragma once
 #include "dense_tile.cuh"
 
@@ -53,6 +54,7 @@ struct DensePairParams {
     int a_mn, b_mn, act, bias_fp32;
     int tma_out, tma_res, save_f32;
     uint32_t idesc;
+    DenseColsum colsum;              // bias gradients to finish beside the product
 };
 
 // ---- CTA-pair forms of the helpers in tc.cuh --------------------------------------------------------------------------
@@ -489,6 +491,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(DP_THREADS, 1)
                 __syncwarp();
             }
         }
+    } else if (warp == 3) {
+        if (MODE != DP_GATED) dense_colsum<HALF>(p.colsum, (int)blockIdx.x, (int)gridDim.x);
     } else if (warp >= 4) {
         if (MODE == DP_PARTIAL) {
             dense_pair_epilogue<MODE, ACT_NONE, HALF, FLAGS>(p, sm, &my, &mr, tmem, rank, t);

@@ -38,6 +38,7 @@ struct DenseTileParams {
     int a_mn, b_mn;                 // operands stored with the reduction as their slow axis
     int act, bias_fp32;
     uint32_t idesc;
+    DenseColsum colsum;             // bias gradients to finish beside the product
 };
 
 __device__ __forceinline__ void tma_load_2d(void *dst_smem, const CUtensorMap *map, int c0, int c1, uint64_t *bar) {
@@ -272,6 +273,8 @@ __global__ void __launch_bounds__(DT_THREADS, 2) dense_tile_kernel(const __grid_
             if (++slot == p.stages) slot = 0, phase ^= 1;
         }
         if (ok && leader) umma_commit(&bar_done);
+    } else if (warp == 3) {
+        dense_colsum<HALF>(p.colsum, (int)(blockIdx.x + gridDim.x * (blockIdx.y + gridDim.y * blockIdx.z)), (int)(gridDim.x * gridDim.y * gridDim.z));
     }
     __syncwarp();
     float b0[4], b1[4];  // (on their way while the products run)
