@@ -410,7 +410,7 @@ enum pai_tune_key {
     PAI_TUNE_DENSE_KERNEL = 9,    /* feed-forward products: 1 = dense_tile_kernel, 2 = dense_pair_kernel, 3 = dense_vec_kernel where it applies (set it before the forward call and leave
                                      it until the backward call has been made: the saved pre-activations go by the kernel) */
     PAI_TUNE_DENSE_WIDTH = 10,    /* with it: rows of a tile (16 .. 256), accumulator columns of a pair's tile (128, 256) */
-    PAI_TUNE_DENSE_SPLITS = 11,   /* with it: split of the reduction (tile: 1, 2, 4, 8; pair: weight gradients only, 1 .. 8) */
+    PAI_TUNE_DENSE_SPLITS = 11,   /* with it: split of the reduction (tile: 1, 2, 4, 8; pair: weight gradients only, 1 .. 64) */
     PAI_TUNE_COUNT = 12
 };
 int pai_tune_set(int key, int value);

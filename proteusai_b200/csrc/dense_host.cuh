@@ -24,7 +24,10 @@ static int make_map_16(CUtensorMap *map, const void *base, long long inner, long
     return r == CUDA_SUCCESS ? 0 : (int)PAI_ERR_UNSUPPORTED;
 }
 
-// Launch as a programmatic dependent of what is on the stream (common.cuh), in clusters of `cluster` CTAs if it is more than 1.
+// Launch as a programmatic dependent of what is on the stream (common.cuh), in clusters of `cluster` CTAs if it is more than 1; cluster 0: in
+// order.  A kernel that lives on plain loads goes in order behind the products: brought onto their SMs early it also inherits their split of
+// the SM's memory, which leaves it next to no L1 for loads in flight (joining 32 tiles of 512 x 256: 33 us for 8; a gated training step of
+// 16384 x 512 x 2048: 245 us for 230).
 template <typename... P, typename... A>
 static int dense_launch_kernel(void (*kernel)(P...), dim3 grid, int block, int smem, cudaStream_t st, int cluster, const A &...args) {
     cudaLaunchConfig_t cfg = {};
@@ -39,7 +42,7 @@ static int dense_launch_kernel(void (*kernel)(P...), dim3 grid, int block, int s
     at[1].val.clusterDim.x = (unsigned)cluster;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cfg.numAttrs = cluster > 1 ? 2 : cluster;
     return (int)cudaLaunchKernelEx(&cfg, kernel, P(args)...);
 }
 
@@ -112,11 +115,12 @@ static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_sp
         if (g_dense_tune.kernel == 2 && g_dense_tune.width && bn != g_dense_tune.width) continue;
         const int fw = d.dual ? bn / 2 : bn;
         const long long tiles = (d.F + fw - 1) / fw * ((d.T + 255) / 256) * d.groups;
-        for (int splits = 1; splits <= (may_split ? 8 : 1) && splits * 4 <= (kb > 4 ? kb : 4); ++splits) {
+        for (int splits = 1; splits <= (may_split ? 64 : 1) && splits * 4 <= (kb > 4 ? kb : 4); ++splits) {
             if (g_dense_tune.kernel == 2 && g_dense_tune.splits && may_split && splits != g_dense_tune.splits) continue;
+            if (splits > 1 && tiles * splits > sms / 2 && g_dense_tune.splits == 0) break;  // (a second round of short items costs more than it saves)
             const double rounds = (double)((tiles * splits + sms / 2 - 1) / (sms / 2)), blocks = (double)((kb + splits - 1) / splits);
             const double tile = bn == 256 ? 0.29 * blocks + 0.46 : 0.237 * blocks;
-            const double t = 3.85 + rounds * tile + 0.287 * out + (splits > 1 ? 1.65 + 1.54 * splits * out : 0.0);
+            const double t = 3.85 + rounds * tile + 0.287 * out + (splits > 1 ? 3.0 + splits * (0.16 + 1.54 * out) : 0.0);
             if (t < best.cost) best = {1, bn, splits, t};
         }
     }
@@ -270,7 +274,7 @@ static int dense_pair_launch(const DenseProduct &d, const DenseChoice &c, int sm
     if (partial) {
         if (int e = d.half ? dense_pair_launch_as<DP_PARTIAL, 1, 0>(m, p, ctas, st) : dense_pair_launch_as<DP_PARTIAL, 0, 0>(m, p, ctas, st)) return e;
         const size_t blocks = saved_blocks(d.T, (int)d.F);
-        return dense_launch_kernel(dense_reduce_kernel, dim3((unsigned)blocks, d.groups), 256, 0, st, 1, d.part, d.out[0], d.out[1], p.T, p.F, d.ld_out,
+        return dense_launch_kernel(dense_reduce_kernel, dim3((unsigned)blocks, d.groups), 256, 0, st, 0, d.part, d.out[0], d.out[1], p.T, p.F, d.ld_out,
                                    d.groups, c.splits, d.half);
     }
     const int any = !p.tma_out || (d.residual && !p.tma_res) ? DP_ANY : 0;
@@ -388,9 +392,9 @@ static size_t dense_bwd_workspace(long long M, int N, int K, int mats, int sms) 
 
 template <bool DUAL, int ACT>
 static int dense_bwd_elem_as(const DenseBwdElemParams &p, int half, bool f32, dim3 grid, cudaStream_t st) {
-    if (half) return dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 1, true>, grid, 256, 0, st, 1, p);
-    return f32 ? dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 0, true>, grid, 256, 0, st, 1, p)
-               : dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 0, false>, grid, 256, 0, st, 1, p);
+    if (half) return dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 1, true>, grid, 256, 0, st, 0, p);
+    return f32 ? dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 0, true>, grid, 256, 0, st, 0, p)
+               : dense_launch_kernel(dense_bwd_elem_kernel<DUAL, ACT, 0, false>, grid, 256, 0, st, 0, p);
 }
 template <bool DUAL>
 static int dense_bwd_elem_act(const DenseBwdElemParams &p, int act, int half, bool f32, dim3 grid, cudaStream_t st) {

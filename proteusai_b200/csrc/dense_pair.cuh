@@ -108,8 +108,13 @@ __device__ __forceinline__ void save_run_f16(uint8_t *values, uint8_t *exps, siz
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) m = fmaxf(m, fabsf(v[i]));
+    if (m > 3.4e38f) {  // an infinity does not set the scale of the others
+        m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = isinf(v[i]) ? m : fmaxf(m, fabsf(v[i]));
+    }
     int e = (int)(__float_as_uint(m) >> 23) - 127 - 14;  // 2^e 2^14 <= m < 2^e 2^15
-    if (m == 0.f || m > 3.4e38f) e = 0;
+    if (m == 0.f) e = 0;
     e = e < -112 ? -112 : e;  // (2^-e stays finite; what is smaller than 2^-98 loses bits)
     const float s = __uint_as_float((uint32_t)(127 - e) << 23);
     uint4 *dst = reinterpret_cast<uint4 *>(values + block * 2048) + ((col & 31) >> 3) * 32 + row;
@@ -529,7 +534,7 @@ __global__ void __launch_bounds__(256) dense_reduce_kernel(const float *__restri
     const int t = (int)(b / col_blocks) * 32 + r, f = (int)(b % col_blocks) * 32 + (lane & 7) * 4;
     const float *src = part + group * matrix + b * 1024 + (lane & 7) * 128 + r * 4;
     float4 s = *reinterpret_cast<const float4 *>(src);
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 1; i < splits; ++i) {
         const float4 v = *reinterpret_cast<const float4 *>(src + (size_t)i * groups * matrix);
         s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
