@@ -75,8 +75,8 @@ struct DenseTune {
 static DenseTune g_dense_tune;
 
 // The kernel and its shape are the ones with the lowest estimated time, in microseconds: models with coefficients fitted to 699 measurements of all
-// shapes at 19 sizes from 16 x 512 x 2048 to 16384 x 512 x 2048, one product after another on a stream (r.m.s. 9 and 7 %; the choice is within
-// 9 % of the best shape on all 76 products).
+// shapes at 19 sizes from 16 x 512 x 2048 to 16384 x 512 x 2048, one product after another on a stream (r.m.s. 9 and 7 %; the cost per split
+// came later, from reductions of up to 65536).  The choice is within 10 % of the best shape measured on all of 83 products.
 struct DenseChoice {
     int pair, width, splits;   // width: rows t of a tile (tile kernel), accumulator columns (pair kernel)
     double cost;
@@ -120,7 +120,7 @@ static DenseChoice dense_pair_choose(const DenseProduct &d, int sms, bool may_sp
             if (splits > 1 && tiles * splits > sms / 2 && g_dense_tune.splits == 0) break;  // (a second round of short items costs more than it saves)
             const double rounds = (double)((tiles * splits + sms / 2 - 1) / (sms / 2)), blocks = (double)((kb + splits - 1) / splits);
             const double tile = bn == 256 ? 0.29 * blocks + 0.46 : 0.237 * blocks;
-            const double t = 3.85 + rounds * tile + 0.287 * out + (splits > 1 ? 3.0 + splits * (0.16 + 1.54 * out) : 0.0);
+            const double t = 3.85 + rounds * tile + 0.287 * out + (splits > 1 ? 1.65 + splits * (0.16 + 1.54 * out) : 0.0);
             if (t < best.cost) best = {1, bn, splits, t};
         }
     }
