@@ -544,6 +544,73 @@ def test_encoder_model_inference_and_training(ffn):
             assert p.grad is not None and torch.isfinite(p.grad).all(), name
 
 
+@pytest.mark.parametrize("m,k,n", [(65536, 64, 64), (40000, 512, 20), (20001, 72, 136)])
+def test_long_reductions_in_many_splits(m, k, n):
+    """Few tiles of weight gradient under a long batch: the reduction is split over many pairs of SMs and joined in order, the same bits every time."""
+    for mats, act in ((1, "silu"), (1, None), (2, "gelu")):
+        x, ws, bs, _, dy = _inputs(m, k, n, torch.bfloat16, mats, True, False, seed=30)
+        got, again = _run(x, ws, bs, None, dy, act), _run(x, ws, bs, None, dy, act)
+        _check(got, _expected(x, ws, bs, None, dy, act), torch.bfloat16, f"{mats} {act}")
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("kernel", (1, 2))
+def test_an_infinity_beside_finite_pre_activations(tuned, kernel):
+    """A pre-activation that overflows does not cost its neighbours in the same saved run their bits: their gradients are as without it."""
+    m, k, n = 256, 64, 256
+    tuned(dense_kernel=kernel)
+    x, ws, _, _, dy = _inputs(m, k, n, torch.bfloat16, 2, False, seed=31)
+    x[:, 0] = 1e38
+    ws = [w.clone() for w in ws]
+    for w in ws:
+        w[:, 0] = 0.0
+    clean = _run(x, ws, [None, None], None, dy, "relu")
+    ws[1][5, 0] = 1e30                               # u is +inf in column 5, z is as before
+    got = _run(x, ws, [None, None], None, dy, "relu")
+    others = torch.arange(n, device="cuda") != 5
+    assert torch.equal(got[0][:, others], clean[0][:, others])
+    for a, b in zip(got[2:], clean[2:]):
+        assert torch.equal(a[others], b[others])
+
+
+def test_a_backward_pass_under_another_tuning_is_refused(tuned):
+    """The saved pre-activations have the form of the kernel that wrote them."""
+    from proteusai_b200.utils.model_utils.base_modules import fused_ops
+    x, ws, _, _, dy = _inputs(512, 64, 256, torch.bfloat16, 2, False, seed=32)
+    for gated in (False, True):
+        tuned(dense_kernel=2)
+        xl = x.clone().requires_grad_(True)
+        y = fused_ops.gated_linear(xl, *ws) if gated else fused_ops.linear(xl, ws[0], act="silu")
+        tuned(dense_kernel=1)
+        with pytest.raises(RuntimeError, match="tuning changed"):
+            y.backward(dy)
+        assert xl.grad is None
+
+
+def test_capture_beside_a_graph_of_the_default_stream_is_refused():
+    from proteusai_b200.utils.model_utils.base_modules import fused_ops
+    x, ws, _, _, dy = _inputs(40, 64, 72, torch.bfloat16, 1, False, seed=33)
+    w = ws[0].clone().requires_grad_(True)
+    alive = fused_ops.linear(x, w)                   # keeps w's accumulator, which belongs to the default stream
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with pytest.raises(RuntimeError, match="being captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+            fused_ops.linear(x, w).backward(dy)
+    assert w.grad is None
+    alive.backward(dy)                               # neither graph nor device came to harm
+    ref = dy.double().t() @ x.double()
+    assert ((w.grad.double() - ref).norm() / ref.norm()).item() <= 2 * 2.0 ** -8
+    del alive
+    w.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        fused_ops.linear(x, w).backward(dy)
+    g.replay()
+    torch.cuda.synchronize()
+    assert ((w.grad.double() - ref).norm() / ref.norm()).item() <= 2 * 2.0 ** -8
+
+
 def test_waits_never_ran_out():
     from proteusai_b200 import _lib
     _lib.device_status()
